@@ -37,7 +37,7 @@ def _nvcc() -> str:
 
 def sources():
     return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh"))) + [
-        os.path.join(os.path.dirname(_HERE), "include", "bittorch_b200.h")
+        os.path.join(os.path.dirname(_HERE), "include", h) for h in ("bittorch_b200.h", "bittorch_b200_cache.h")
     ]
 
 

@@ -1,0 +1,334 @@
+"""ctypes binding of the operators over a key/value cache (include/bittorch_b200_cache.h), and their argument checks.
+
+The entry points live in the same library as ``_C``'s; they are bound here, on first use, so that a caller of the
+linear layers alone needs none of them.  Shapes and types are checked before devices, with messages as
+``RuntimeError``; nothing here computes on the CPU.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Sequence, Tuple
+
+import torch
+from torch import Tensor
+
+from . import _C
+
+_p, _i64, _int, _f32, _size = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
+
+BEAM_MAX_SELECT = 64
+BEAM_MAX_BEAMS = 64
+REORDER_MAX_BEAMS = 32
+ATTENTION_MAX_HEAD_DIM = 256
+
+_SIGNATURES = {
+    "bt_tree_attention_workspace": ([_i64] * 6 + [_int, _int], _size),
+    "bt_tree_attention": ([_p, _p, _p, _int] + [_i64] * 6 + [_p, _p, _int, _i64, _p, _i64, _f32, _p, _i64, _i64, _p, _p, _size, _p], _int),
+    "bt_evict_select": ([_p, _i64, _i64, _i64, _i64, _i64, _p, _int, _i64, _i64, _i64, _i64, _p, _p, _p], _int),
+    "bt_compact_cache": ([_p, _p, _p, _p, _int] + [_i64] * 5 + [_p, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p], _int),
+    "bt_beam_select_workspace": ([_i64, _i64, _i64, _int, _i64], _size),
+    "bt_beam_select": ([_p, _int] + [_i64] * 5 + [_p, _p, _i64, _i64, _p, _p, _p, _p, _size, _p], _int),
+    "bt_reorder_cache": ([_p, _i64, _int] + [_i64] * 5 + [_p, _p, _p, _int, _i64, _i64, _p], _int),
+}
+EXPORTED = tuple(_SIGNATURES)
+
+
+def _bind():
+    fns = {}
+    for name, (argtypes, restype) in _SIGNATURES.items():
+        try:
+            fn = getattr(_C._lib, name)
+        except AttributeError as exc:
+            raise ImportError(f"bittorch_b200: {_C.LIB_PATH} is stale (no symbol {name}); rebuild it with "
+                              "`python -m bittorch_b200._build`") from exc
+        fn.argtypes, fn.restype = argtypes, restype
+        fns[name] = fn
+    return fns
+
+
+_fn = _bind()
+_tree_attention, _tree_attention_workspace = _fn["bt_tree_attention"], _fn["bt_tree_attention_workspace"]
+_evict_select, _compact_cache = _fn["bt_evict_select"], _fn["bt_compact_cache"]
+_beam_select, _beam_select_workspace = _fn["bt_beam_select"], _fn["bt_beam_select_workspace"]
+_reorder_cache = _fn["bt_reorder_cache"]
+
+_DT = _C._DT
+_SIX, _TWELVE, _FOUR = _i64 * 6, _i64 * 12, _i64 * 4
+
+
+def _fail(text: str):
+    raise RuntimeError(text)
+
+
+def _require(ok: bool, text: str) -> None:
+    if not ok:
+        raise RuntimeError(text)
+
+
+def _no_gradient(what: str, *tensors: Optional[Tensor]) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        _fail(f"{what} has no backward pass: call it under torch.no_grad()")
+
+
+def _on_one_device(what: str, *tensors: Optional[Tensor]) -> torch.device:
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None:
+            if not t.is_cuda:
+                _fail("All tensors must be CUDA")
+            if t.device != dev:
+                _fail(f"{what}: all tensors must be on one device")
+    return dev
+
+
+def _plain_memory(t: Tensor) -> bool:
+    """No two elements of ``t`` share memory (what is written in place must not)."""
+    if t.is_contiguous():
+        return True
+    span = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz > 1):
+        if stride < span:
+            return False
+        span = stride * size
+    return True
+
+
+def _call(dev: torch.device, fn, *args) -> None:
+    """Enqueue on the current stream of ``dev``."""
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if rc:
+        _C._check(rc)
+
+
+def _lengths(lengths: Tensor, batch: int) -> Tuple[int, int]:
+    """(is int64, stride): one length for the batch, or one per sequence."""
+    if lengths.dim() != 1 or lengths.shape[0] not in (1, batch):
+        _fail(f"lengths must be [{batch}] or [1], got {list(lengths.shape)}")
+    if lengths.dtype is not torch.int64 and lengths.dtype is not torch.int32:
+        _fail(f"lengths must be int64 or int32, got {lengths.dtype}")
+    return (1 if lengths.dtype is torch.int64 else 0), (0 if lengths.shape[0] == 1 else lengths.stride(0))
+
+
+def _cache_pair(what: str, k: Tensor, v: Tensor) -> None:
+    if k.dim() != 4 or k.shape != v.shape:
+        _fail(f"{what}: keys and values must be 4D [B, Hkv, S, D] of one shape")
+    if k.dtype != v.dtype or k.dtype not in _DT:
+        _fail(f"{what}: keys and values must both be float32, float16 or bfloat16, got {k.dtype} and {v.dtype}")
+    if k.numel() == 0:
+        _fail(f"{what}: the cache is empty")
+    if (k.stride(3) != 1 or v.stride(3) != 1) and k.shape[3] != 1:
+        _fail(f"{what}: the head dimension of a cache must be contiguous")
+
+
+def tree_attention(q: Tensor, k: Tensor, v: Tensor, lengths: Tensor, tree: Optional[Tensor], scale: Optional[float],
+                   mass: Optional[Tensor], out: Optional[Tensor]) -> Tensor:
+    if q.dim() != 4:
+        _fail("q must be 4D [B, H, T, D]")
+    b, h, t, d = q.shape
+    _cache_pair("tree_attention", k, v)
+    if q.dtype != k.dtype:
+        _fail(f"q must have the cache's type {k.dtype}, got {q.dtype}")
+    if k.shape[0] != b or k.shape[3] != d:
+        _fail(f"q {list(q.shape)} and the cache {list(k.shape)} differ in batch or head size")
+    hkv, s = k.shape[1], k.shape[2]
+    if q.numel() == 0:
+        _fail("q is empty")
+    if h % hkv:
+        _fail(f"{h} query heads are not a multiple of {hkv} key/value heads")
+    if d > ATTENTION_MAX_HEAD_DIM:
+        _fail(f"head sizes up to {ATTENTION_MAX_HEAD_DIM} are supported, got {d}")
+    if t > s:
+        _fail(f"{t} new tokens do not fit a cache of {s} slots")
+    len64, len_stride = _lengths(lengths, b)
+    tree_sb = 0
+    if tree is not None:
+        if tree.dtype is not torch.bool or tuple(tree.shape) not in ((t, t), (b, t, t)):
+            _fail(f"tree must be bool [{t}, {t}] or [{b}, {t}, {t}], got {tree.dtype} {list(tree.shape)}")
+        tree_sb = t * t if tree.dim() == 3 else 0
+    if scale is None:
+        scale = 1.0 / math.sqrt(d)
+    elif not math.isfinite(scale):
+        _fail("scale must be finite")
+    if mass is not None:
+        if mass.dtype is not torch.float32 or mass.shape != k.shape[:3]:
+            _fail(f"mass must be float32 {list(k.shape[:3])}, got {mass.dtype} {list(mass.shape)}")
+        if (mass.stride(2) != 1 and s != 1) or not _plain_memory(mass):
+            _fail("mass must have contiguous slots that share no memory")
+    if out is not None:
+        if out.shape != q.shape or out.dtype != q.dtype:
+            _fail(f"out must be {q.dtype} {list(q.shape)}, got {out.dtype} {list(out.shape)}")
+        if (out.stride(3) != 1 and d != 1) or not _plain_memory(out):
+            _fail("out must have a contiguous head dimension and share no memory with itself")
+    _no_gradient("tree_attention", q, k, v, mass, out)
+    dev = _on_one_device("tree_attention", q, k, v, lengths, tree, mass, out)
+    if q.stride(3) != 1:
+        q = q.contiguous()
+    if tree is not None and not tree.is_contiguous():
+        tree = tree.contiguous()
+    if out is None:                       # the layout of the projection that follows: [B, T, H * D]
+        out = torch.empty((b, t, h, d), dtype=q.dtype, device=dev).transpose(1, 2)
+    code = _DT[q.dtype]
+    need = _workspace_bytes(dev, b, h, hkv, t, s, d, code, mass is not None)
+    work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    strides = _TWELVE(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3])
+    mass_sb, mass_sh = (0, 0) if mass is None else mass.stride()[:2]
+    _call(dev, _tree_attention, q.data_ptr(), k.data_ptr(), v.data_ptr(), code, b, h, hkv, t, s, d, strides,
+          lengths.data_ptr(), len64, len_stride, None if tree is None else tree.data_ptr(), tree_sb, scale,
+          None if mass is None else mass.data_ptr(), mass_sb, mass_sh, out.data_ptr(),
+          None if work is None else work.data_ptr(), need)
+    return out
+
+
+def _workspace_bytes(dev: torch.device, *sizes) -> int:
+    if dev.index == torch.cuda.current_device():       # it depends on the device's SM count
+        return _tree_attention_workspace(*sizes)
+    with torch.cuda.device(dev):
+        return _tree_attention_workspace(*sizes)
+
+
+def evict_select(mass: Tensor, lengths: Tensor, budget: int, sinks: int, recent: int) -> Tuple[Tensor, Tensor]:
+    if mass.dim() != 3 or mass.dtype is not torch.float32 or mass.numel() == 0:
+        _fail(f"mass must be float32 [B, Hkv, S], got {mass.dtype} {list(mass.shape)}")
+    if mass.stride(2) != 1 and mass.shape[2] != 1:
+        _fail("mass must have contiguous slots")
+    b, hkv, s = mass.shape
+    budget, sinks, recent = int(budget), int(sinks), int(recent)
+    if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
+        _fail(f"a budget of {budget} slots must be positive and hold {sinks} sinks and {recent} recent slots")
+    len64, len_stride = _lengths(lengths, b)
+    dev = _on_one_device("evict_select", mass, lengths)
+    keep = torch.empty((b, hkv, budget), dtype=torch.int64, device=dev)
+    counts = torch.empty((b,), dtype=torch.int64, device=dev)
+    _call(dev, _evict_select, mass.data_ptr(), mass.stride(0), mass.stride(1), b, hkv, s, lengths.data_ptr(), len64, len_stride,
+          budget, sinks, recent, keep.data_ptr(), counts.data_ptr())
+    return keep, counts
+
+
+def compact_cache(k: Tensor, v: Tensor, keep: Tensor, counts: Tensor, first: Optional[Tensor], mass: Optional[Tensor],
+                  out: Optional[Sequence[Tensor]]) -> None:
+    _cache_pair("compact_cache", k, v)
+    b, hkv, s, d = k.shape
+    if out is None:
+        k_out, v_out, mass_out = k, v, mass
+    else:
+        if len(out) != (2 if mass is None else 3):
+            _fail("out must be (keys, values), with the mass third where one is given")
+        k_out, v_out, mass_out = out[0], out[1], (out[2] if mass is not None else None)
+        _cache_pair("compact_cache", k_out, v_out)
+        if k_out.dtype != k.dtype or k_out.shape[:2] != k.shape[:2] or k_out.shape[3] != d:
+            _fail(f"out must be {k.dtype} [{b}, {hkv}, slots, {d}], got {k_out.dtype} {list(k_out.shape)}")
+        if k_out.data_ptr() in (k.data_ptr(), v.data_ptr()) or v_out.data_ptr() in (k.data_ptr(), v.data_ptr(), k_out.data_ptr()):
+            _fail("out must be other memory than the cache (leave it out to compact in place)")
+    s_out = k_out.shape[2]
+    if keep.dim() != 3 or keep.dtype is not torch.int64 or keep.shape[0] != b or keep.shape[1] not in (1, hkv) or keep.shape[2] == 0:
+        _fail(f"keep must be int64 [{b}, {hkv} or 1, n], got {keep.dtype} {list(keep.shape)}")
+    for name, t in (("counts", counts), ("first", first)):
+        if t is not None and (t.dtype is not torch.int64 or tuple(t.shape) != (b,)):
+            _fail(f"{name} must be int64 [{b}], got {t.dtype} {list(t.shape)}")
+    if mass is not None:
+        for m, slots in ((mass, s), (mass_out, s_out)):
+            if m.dtype is not torch.float32 or tuple(m.shape) != (b, hkv, slots) or (m.stride(2) != 1 and slots != 1):
+                _fail(f"mass must be float32 [{b}, {hkv}, {slots}] with contiguous slots, got {m.dtype} {list(m.shape)}")
+        if out is not None and mass_out.data_ptr() == mass.data_ptr():
+            _fail("out must be other memory than the mass (leave it out to compact in place)")
+    if not (_plain_memory(k_out) and _plain_memory(v_out) and (mass_out is None or _plain_memory(mass_out))):
+        _fail("compact_cache: what is written must share no memory with itself")
+    _no_gradient("compact_cache", k, v, k_out, v_out, mass, mass_out)
+    dev = _on_one_device("compact_cache", k, v, k_out, v_out, keep, counts, first, mass, mass_out)
+    if keep.stride(2) != 1:
+        keep = keep.contiguous()
+    counts = counts.contiguous()
+    first = None if first is None else first.contiguous()
+    strides = _TWELVE(*k.stride()[:3], *v.stride()[:3], *k_out.stride()[:3], *v_out.stride()[:3])
+    mass_strides = None if mass is None else _FOUR(*mass.stride()[:2], *mass_out.stride()[:2])
+    _call(dev, _compact_cache, k.data_ptr(), v.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), _DT[k.dtype], b, hkv, s, s_out, d,
+          strides, keep.data_ptr(), keep.stride(0), keep.stride(1) if keep.shape[1] == hkv else 0, keep.shape[2],
+          counts.data_ptr(), None if first is None else first.data_ptr(), None if mass is None else mass.data_ptr(),
+          None if mass is None else mass_out.data_ptr(), mass_strides)
+
+
+def beam_select(logits: Tensor, scores: Tensor, select: Optional[int], finished: Optional[Tensor],
+                end_token: Optional[int]) -> Tuple[Tensor, Tensor, Tensor]:
+    if logits.dim() != 3 or logits.dtype not in _DT:
+        _fail(f"logits must be float32, float16 or bfloat16 [B, beams, vocabulary], got {logits.dtype} {list(logits.shape)}")
+    b, w, vocab = logits.shape
+    if logits.numel() == 0:
+        _fail("logits are empty")
+    n = w if select is None else int(select)
+    if scores.dtype is not torch.float32 or scores.shape != (b, w):
+        _fail(f"scores must be float32 [{b}, {w}], got {scores.dtype} {list(scores.shape)}")
+    if not 1 <= w <= BEAM_MAX_BEAMS:
+        _fail(f"up to {BEAM_MAX_BEAMS} beams are supported, got {w}")
+    if not 1 <= n <= min(BEAM_MAX_SELECT, w * vocab):
+        _fail(f"select must be 1 to {min(BEAM_MAX_SELECT, w * vocab)}, got {n}")
+    if (finished is None) != (end_token is None):
+        _fail("finished and end_token come together")
+    if finished is not None:
+        if finished.dtype is not torch.bool or finished.shape != (b, w):
+            _fail(f"finished must be bool [{b}, {w}], got {finished.dtype} {list(finished.shape)}")
+        if not 0 <= end_token < vocab:
+            _fail(f"end_token {end_token} is outside the vocabulary of {vocab}")
+    _no_gradient("beam_select", logits, scores)
+    dev = _on_one_device("beam_select", logits, scores, finished)
+    if logits.stride(2) != 1:
+        logits = logits.contiguous()
+    scores = scores.contiguous()
+    finished = None if finished is None else finished.contiguous()
+    code = _DT[logits.dtype]
+    need = _beam_select_workspace(b, w, vocab, code, n)
+    out = torch.empty((b, n), dtype=torch.float32, device=dev)
+    picks = torch.empty((2, b, n), dtype=torch.int64, device=dev)
+    work = torch.empty(need, dtype=torch.uint8, device=dev)
+    tokens, parents = picks[0], picks[1]
+    _call(dev, _beam_select, logits.data_ptr(), code, b, w, vocab, logits.stride(0), logits.stride(1), scores.data_ptr(),
+          None if finished is None else finished.data_ptr(), 0 if end_token is None else int(end_token), n, out.data_ptr(),
+          tokens.data_ptr(), parents.data_ptr(), work.data_ptr(), need)
+    return out, tokens, parents
+
+
+def reorder_cache(caches: Sequence[Tensor], parents: Tensor, lengths: Tensor, start: int) -> None:
+    if len(caches) == 0:
+        _fail("reorder_cache: no cache tensors")
+    if parents.dim() != 2 or parents.dtype is not torch.int64 or parents.numel() == 0:
+        _fail(f"parents must be int64 [B, beams], got {parents.dtype} {list(parents.shape)}")
+    b, w = parents.shape
+    if w > REORDER_MAX_BEAMS:
+        _fail(f"up to {REORDER_MAX_BEAMS} beams are supported, got {w}")
+    shape, dtype = caches[0].shape, caches[0].dtype
+    if len(shape) != 4 or shape[0] != b * w or caches[0].numel() == 0 or dtype not in _DT:
+        _fail(f"cache tensors must be float32, float16 or bfloat16 [{b * w}, Hkv, S, D], got {dtype} {list(shape)}")
+    start = int(start)
+    _require(start >= 0, "start must not be negative")
+    len64, len_stride = _lengths(lengths, b)
+    dev = parents.device
+    pointers, strides = [], []
+    contiguous = True
+    grad = torch.is_grad_enabled()
+    for c in caches:
+        if c.shape != shape or c.dtype != dtype:
+            _fail("reorder_cache: all cache tensors must have one shape and type")
+        st = c.stride()
+        if not c.is_contiguous():
+            contiguous = False
+            if (st[3] != 1 and shape[3] != 1) or not _plain_memory(c):
+                _fail("reorder_cache: cache tensors must have a contiguous head dimension and share no memory with themselves")
+        if grad and c.requires_grad:
+            _no_gradient("reorder_cache", c)
+        pointers.append(c.data_ptr())
+        strides += st[:3]
+    _on_one_device("reorder_cache", parents, lengths, *caches)
+    if len(set(pointers)) < len(pointers):
+        _fail("reorder_cache: a cache tensor is listed twice")
+    if contiguous and len(pointers) > 1:
+        ordered, size = sorted(pointers), caches[0].numel() * caches[0].element_size()
+        _require(all(y - x >= size for x, y in zip(ordered, ordered[1:])), "reorder_cache: cache tensors share memory")
+    parents = parents.contiguous()
+    count = len(pointers)
+    _call(dev, _reorder_cache, (_p * count)(*pointers), count, _DT[dtype], b, w, shape[1], shape[2], shape[3],
+          (_i64 * (3 * count))(*strides), parents.data_ptr(), lengths.data_ptr(), len64, len_stride, start)

@@ -65,6 +65,10 @@ __global__ void wait_timeout_selftest_kernel(int polls) {
 }  // namespace bt
 
 #include "act_quant.cuh"
+#include "beam_select.cuh"
+#include "cache_attention.cuh"
+#include "cache_evict.cuh"
+#include "cache_reorder.cuh"
 #include "float_planes.cuh"
 #include "fused_elementwise.cuh"
 #include "gemm_tcgen05.cuh"
