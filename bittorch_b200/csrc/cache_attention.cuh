@@ -295,8 +295,8 @@ static AttnPlan attn_plan(int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t 
     const int64_t rows = H / Hkv * T;
     a.row_tiles = static_cast<int>(ceil_div<int64_t>(rows, AT_ROWS));
     const int64_t units = B * Hkv * a.row_tiles;
-    // about four CTAs per SM, no run shorter than one unit of a full cache
-    int64_t split = ceil_div<int64_t>(static_cast<int64_t>(sm_count()) * 4, units);
+    // about eight CTAs per SM, no run shorter than one unit of a full cache
+    int64_t split = ceil_div<int64_t>(static_cast<int64_t>(sm_count()) * 8, units);
     split = std::min<int64_t>(split, ceil_div<int64_t>(S, AT_UNIT));
     a.nsplit = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(split, AT_MAX_SPLIT)));
     const size_t all = static_cast<size_t>(B) * Hkv * rows;
@@ -307,13 +307,26 @@ static AttnPlan attn_plan(int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t 
     return a;
 }
 
+// cache_attention_stream.cuh
+static bool attn_stream_ok(const AttnParams& p);
+template <typename T> static int launch_attn_stream_for(const AttnParams& p, void* stream);
+
 template <typename T>
-static int launch_attention(const AttnParams& p, const AttnPlan& plan, void* stream) {
+static int launch_attn_split(const AttnParams& p, void* stream) {
+#ifndef BT_SIMT_HOST
+    if constexpr (sizeof(T) == 2)
+        if (attn_stream_ok(p)) return launch_attn_stream_for<T>(p, stream);
+#endif
     const size_t smem = attn_smem(p.D);
     static std::atomic<size_t> granted[BT_MAX_DEVICES];
     if (const int rc = ensure_dynamic_smem(attn_split_kernel<T>, smem, granted)) return rc;
     const int64_t ctas = static_cast<int64_t>(p.B) * p.Hkv * p.row_tiles * p.nsplit;
-    if (const int rc = launch_early(attn_split_kernel<T>, "attn_split_kernel", dim3(static_cast<unsigned>(ctas)), AT_THREADS, smem, stream, p)) return rc;
+    return launch_early(attn_split_kernel<T>, "attn_split_kernel", dim3(static_cast<unsigned>(ctas)), AT_THREADS, smem, stream, p);
+}
+
+template <typename T>
+static int launch_attention(const AttnParams& p, const AttnPlan& plan, void* stream) {
+    if (const int rc = launch_attn_split<T>(p, stream)) return rc;
     if (plan.ml_bytes == 0) return BT_OK;
     const int64_t rows = static_cast<int64_t>(p.B) * p.Hkv * p.rows;
     int64_t blocks = p.nsplit > 1 ? ceil_div<int64_t>(rows, AT_THREADS / 32) : 0;

@@ -67,6 +67,7 @@ __global__ void wait_timeout_selftest_kernel(int polls) {
 #include "act_quant.cuh"
 #include "beam_select.cuh"
 #include "cache_attention.cuh"
+#include "cache_attention_stream.cuh"
 #include "cache_evict.cuh"
 #include "cache_reorder.cuh"
 #include "float_planes.cuh"
