@@ -22,6 +22,9 @@ constexpr int AT_ROWS = 16;                      // rows of a CTA
 constexpr int AT_KEYS = 32;                      // slots of a step
 constexpr int AT_UNIT = 64;                      // runs are multiples of this many slots
 constexpr int AT_MAX_SPLIT = 64;
+#ifndef AT_FACTOR
+#define AT_FACTOR 8
+#endif
 
 struct AttnParams {
     const void *q, *k, *v;
@@ -51,6 +54,15 @@ __device__ __forceinline__ void attn_run(int end, int nsplit, int i, int& first,
     const int64_t lo = static_cast<int64_t>(i) * per * AT_UNIT, hi = lo + static_cast<int64_t>(per) * AT_UNIT;
     first = static_cast<int>(lo < end ? lo : end);
     last = static_cast<int>(hi < end ? hi : end);
+}
+// What a CTA of the split kernels works on: splits vary fastest, so that a head's runs are read at the same time
+__device__ __forceinline__ void attn_place(const AttnParams& p, int& split, int& r0, int& h, int& b) {
+    unsigned at = blockIdx.x, next = at / p.nsplit;
+    split = static_cast<int>(at - next * p.nsplit);
+    at = next, next = at / p.row_tiles;
+    r0 = static_cast<int>(at - next * p.row_tiles) * AT_ROWS;
+    b = static_cast<int>(next / p.Hkv);
+    h = static_cast<int>(next - b * p.Hkv);
 }
 // Does token t of sequence b see slot n (n < end)?
 __device__ __forceinline__ bool attn_sees(const AttnParams& p, int b, int len, int t, int n) {
@@ -84,10 +96,8 @@ __global__ void __launch_bounds__(AT_THREADS) attn_split_kernel(const AttnParams
     float* s_alpha = s_p + AT_KEYS * AT_ROWS;                      // [rows]
     float* s_l = s_alpha + AT_ROWS;                                // [rows]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    int64_t at = blockIdx.x;
-    const int split = static_cast<int>(at % p.nsplit); at /= p.nsplit;
-    const int r0 = static_cast<int>(at % p.row_tiles) * AT_ROWS; at /= p.row_tiles;
-    const int h = static_cast<int>(at % p.Hkv), b = static_cast<int>(at / p.Hkv);
+    int split, r0, h, b;
+    attn_place(p, split, r0, h, b);
     pdl_launch_dependents();
     pdl_wait();
     const int len = attn_len(p, b), end = attn_end(p, len);
@@ -217,64 +227,100 @@ __global__ void __launch_bounds__(AT_THREADS) attn_split_kernel(const AttnParams
     }
 }
 
-// Joins the runs of a row: one warp per row.  CTAs past the rows add the rows' weights to the mass, one thread per slot.
+// What a row's runs add up to: the lanes of a warp share them out.  Returns the common maximum (0 for a row that sees
+// nothing), the sum in `l`, and leaves every run's weight exp2(its maximum - the common one) in weight[0 .. nsplit).
+__device__ __forceinline__ float attn_row_stats(const float2* ml, int nsplit, float* weight, float& l) {
+    const int lane = threadIdx.x & 31;
+    float2 mine[AT_MAX_SPLIT / 32];
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < AT_MAX_SPLIT / 32; ++i) {
+        mine[i] = lane + 32 * i < nsplit ? ml[lane + 32 * i] : make_float2(-INFINITY, 0.0f);
+        m = fmaxf(m, mine[i].x);
+    }
+    m = warp_max(m);
+    if (m == -INFINITY) m = 0.0f;
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < AT_MAX_SPLIT / 32; ++i) {
+        const float w = exp2f(mine[i].x - m);
+        l += w * mine[i].y;
+        if (weight != nullptr && lane + 32 * i < nsplit) weight[lane + 32 * i] = mine[i].y == 0.0f ? 0.0f : w;    // 0: wrote nothing
+    }
+    l = warp_add(l);
+    return m;
+}
+
+constexpr int AM_THREADS = 256;
+constexpr int AM_WARPS = AM_THREADS / 32;
+constexpr int AM_ROWS = 64;                      // rows whose statistics a mass CTA holds at a time
+
+// Joins the runs of a row: one warp per row, four columns per lane, the runs' loads independent of one another.  CTAs past
+// the rows add the rows' weights to the mass, one thread per slot.
 template <typename T>
-__global__ void __launch_bounds__(AT_THREADS) attn_merge_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(AM_THREADS) attn_merge_kernel(const AttnParams p) {
+    __shared__ float s_weight[AM_WARPS][AT_MAX_SPLIT];
+    __shared__ float s_m[AM_ROWS], s_inv[AM_ROWS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const unsigned rows = static_cast<unsigned>(p.B) * p.Hkv * p.rows;
+    const unsigned row_blocks = p.nsplit > 1 ? (rows + AM_WARPS - 1) / AM_WARPS : 0;
     pdl_launch_dependents();
     pdl_wait();
-    const int64_t rows = static_cast<int64_t>(p.B) * p.Hkv * p.rows;
-    const int64_t row_blocks = p.nsplit > 1 ? (rows + AT_THREADS / 32 - 1) / (AT_THREADS / 32) : 0;
     if (blockIdx.x < row_blocks) {
-        const int64_t row = blockIdx.x * static_cast<int64_t>(AT_THREADS / 32) + warp;
-        if (row >= rows) return;
-        const int r = static_cast<int>(row % p.rows), h = static_cast<int>(row / p.rows % p.Hkv), b = static_cast<int>(row / p.rows / p.Hkv);
-        const float2* ml = p.part_ml + row * p.nsplit;
-        float m = -INFINITY;
-        for (int i = lane; i < p.nsplit; i += 32) m = fmaxf(m, ml[i].x);
-        m = warp_max(m);
-        const float ref = m == -INFINITY ? 0.0f : m;
-        float l = 0.0f;
-        for (int i = lane; i < p.nsplit; i += 32) l += exp2f(ml[i].x - ref) * ml[i].y;
-        l = warp_add(l);
+        const unsigned row = blockIdx.x * AM_WARPS + warp;
+        if (row >= rows) return;                                   // a whole warp
+        const unsigned bh = row / p.rows;
+        const int r = static_cast<int>(row - bh * p.rows), h = static_cast<int>(bh % p.Hkv), b = static_cast<int>(bh / p.Hkv);
+        float l;
+        attn_row_stats(p.part_ml + static_cast<int64_t>(row) * p.nsplit, p.nsplit, s_weight[warp], l);
+        __syncwarp();
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float* part = p.part_o + static_cast<int64_t>(row) * p.nsplit * p.D;
         T* out = attn_out_row<T>(p, b, h, r);
-        for (int d = lane; d < p.D; d += 32) {
-            float o = 0.0f;
+        const bool wide = p.D % 4 == 0;
+        for (int d = lane * 4; d < p.D; d += 128) {
+            float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
             for (int i = 0; i < p.nsplit; ++i) {
-                const float2 s = ml[i];
-                if (s.y == 0.0f) continue;                         // an empty run wrote nothing
-                o = fmaf(exp2f(s.x - ref), p.part_o[(row * p.nsplit + i) * p.D + d], o);
+                const float w = s_weight[warp][i];
+                if (w == 0.0f) continue;                           // nothing was written there, or it counts for nothing
+                if (wide) {
+                    const float4 x = *reinterpret_cast<const float4*>(part + static_cast<int64_t>(i) * p.D + d);
+                    o[0] = fmaf(w, x.x, o[0]); o[1] = fmaf(w, x.y, o[1]); o[2] = fmaf(w, x.z, o[2]); o[3] = fmaf(w, x.w, o[3]);
+                } else {
+                    for (int e = 0; e < 4; ++e)
+                        if (d + e < p.D) o[e] = fmaf(w, part[static_cast<int64_t>(i) * p.D + d + e], o[e]);
+                }
             }
-            out[d] = from_float<T>(l == 0.0f ? 0.0f : o / l);
+            for (int e = 0; e < 4; ++e)
+                if (d + e < p.D) out[d + e] = from_float<T>(l == 0.0f ? 0.0f : o[e] * inv);
         }
         return;
     }
     // mass[n] += sum over the rows of exp2(score - row's log-sum)
-    const int slot_blocks = (p.S + AT_THREADS - 1) / AT_THREADS;
-    const int64_t at = blockIdx.x - row_blocks;
-    const int h = static_cast<int>(at / slot_blocks % p.Hkv), b = static_cast<int>(at / slot_blocks / p.Hkv);
-    const int n0 = static_cast<int>(at % slot_blocks) * AT_THREADS;
+    const unsigned slot_blocks = (p.S + AM_THREADS - 1) / AM_THREADS;
+    const unsigned at = blockIdx.x - row_blocks, bh = at / slot_blocks;
+    const int h = static_cast<int>(bh % p.Hkv), b = static_cast<int>(bh / p.Hkv);
+    const int n0 = static_cast<int>(at - bh * slot_blocks) * AM_THREADS;
     const int end = attn_end(p, attn_len(p, b));
     if (n0 >= end) return;                                         // for every thread of the CTA
-    __shared__ float s_m[AT_THREADS], s_inv[AT_THREADS];
     const int n = n0 + tid;
     float sum = 0.0f;
-    for (int r0 = 0; r0 < p.rows; r0 += AT_THREADS) {
+    for (int r0 = 0; r0 < p.rows; r0 += AM_ROWS) {
+        const int count = min(AM_ROWS, p.rows - r0);
         __syncthreads();
-        const int r = r0 + tid;
-        if (r < p.rows) {
-            const float2* ml = p.part_ml + attn_row_index(p, b, h, r) * p.nsplit;
-            float m = -INFINITY, l = 0.0f;
-            for (int i = 0; i < p.nsplit; ++i) m = fmaxf(m, ml[i].x);
-            const float ref = m == -INFINITY ? 0.0f : m;
-            for (int i = 0; i < p.nsplit; ++i) l += exp2f(ml[i].x - ref) * ml[i].y;
-            s_m[tid] = ref;
-            s_inv[tid] = l == 0.0f ? 0.0f : 1.0f / l;
+        for (int i = warp; i < count; i += AM_WARPS) {
+            float l;
+            const float m = attn_row_stats(p.part_ml + attn_row_index(p, b, h, r0 + i) * p.nsplit, p.nsplit, nullptr, l);
+            if (lane == 0) {
+                s_m[i] = m;
+                s_inv[i] = l == 0.0f ? 0.0f : 1.0f / l;
+            }
         }
         __syncthreads();
         if (n < end) {
             const float* s = p.scores + attn_row_index(p, b, h, r0) * p.S + n;
-            const int count = min(AT_THREADS, p.rows - r0);
+#pragma unroll 8
             for (int i = 0; i < count; ++i) sum += exp2f(s[static_cast<int64_t>(i) * p.S] - s_m[i]) * s_inv[i];
         }
     }
@@ -296,7 +342,7 @@ static AttnPlan attn_plan(int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t 
     a.row_tiles = static_cast<int>(ceil_div<int64_t>(rows, AT_ROWS));
     const int64_t units = B * Hkv * a.row_tiles;
     // about eight CTAs per SM, no run shorter than one unit of a full cache
-    int64_t split = ceil_div<int64_t>(static_cast<int64_t>(sm_count()) * 8, units);
+    int64_t split = ceil_div<int64_t>(static_cast<int64_t>(sm_count()) * AT_FACTOR, units);
     split = std::min<int64_t>(split, ceil_div<int64_t>(S, AT_UNIT));
     a.nsplit = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(split, AT_MAX_SPLIT)));
     const size_t all = static_cast<size_t>(B) * Hkv * rows;
@@ -329,9 +375,9 @@ static int launch_attention(const AttnParams& p, const AttnPlan& plan, void* str
     if (const int rc = launch_attn_split<T>(p, stream)) return rc;
     if (plan.ml_bytes == 0) return BT_OK;
     const int64_t rows = static_cast<int64_t>(p.B) * p.Hkv * p.rows;
-    int64_t blocks = p.nsplit > 1 ? ceil_div<int64_t>(rows, AT_THREADS / 32) : 0;
-    if (p.mass) blocks += static_cast<int64_t>(p.B) * p.Hkv * ceil_div(p.S, AT_THREADS);
-    return launch_early(attn_merge_kernel<T>, "attn_merge_kernel", dim3(static_cast<unsigned>(blocks)), AT_THREADS, 0, stream, p);
+    int64_t blocks = p.nsplit > 1 ? ceil_div<int64_t>(rows, AM_WARPS) : 0;
+    if (p.mass) blocks += static_cast<int64_t>(p.B) * p.Hkv * ceil_div(p.S, AM_THREADS);
+    return launch_early(attn_merge_kernel<T>, "attn_merge_kernel", dim3(static_cast<unsigned>(blocks)), AM_THREADS, 0, stream, p);
 }
 
 static bool attn_sizes_ok(int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t S, int64_t D) {

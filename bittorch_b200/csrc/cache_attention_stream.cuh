@@ -93,15 +93,18 @@ __global__ void __launch_bounds__(AS_WARPS * 32, 2) attn_stream_kernel(const Att
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     float2* s_ml = reinterpret_cast<float2*>(smem + AS_WARPS * AS_STAGES * STAGE);       // [warps][rows]
     const uint32_t ring = smem_u32(smem) + warp * AS_STAGES * STAGE;
-    int64_t at = blockIdx.x;
-    const int split = static_cast<int>(at % p.nsplit); at /= p.nsplit;
-    const int r0 = static_cast<int>(at % p.row_tiles) * AT_ROWS; at /= p.row_tiles;
-    const int h = static_cast<int>(at % p.Hkv), b = static_cast<int>(at / p.Hkv);
+    int split, r0, h, b;
+    attn_place(p, split, r0, h, b);
     pdl_launch_dependents();
     pdl_wait();
     const int len = attn_len(p, b), end = attn_end(p, len);
     int first, last;
     attn_run(end, p.nsplit, split, first, last);
+    if (first >= last && p.nsplit > 1) {                           // a run that this length does not have
+        const int r = r0 + threadIdx.x;
+        if (threadIdx.x < AT_ROWS && r < p.rows) p.part_ml[attn_row_index(p, b, h, r) * p.nsplit + split] = make_float2(-INFINITY, 0.0f);
+        return;
+    }
     const T* kbase = static_cast<const T*>(p.k) + b * p.kb + h * p.kh;
     const T* vbase = static_cast<const T*>(p.v) + b * p.vb + h * p.vh;
 
@@ -299,17 +302,23 @@ __global__ void __launch_bounds__(AS_WARPS * 32, 2) attn_stream_kernel(const Att
         m_all[0] = fmaxf(m_all[0], s_ml[i * AT_ROWS + g].x);
         m_all[1] = fmaxf(m_all[1], s_ml[i * AT_ROWS + g + 8].x);
     }
-    const float fa = exp2_fast(ma - m_all[0]), fb = exp2_fast(mb - m_all[1]);       // of no meaning where the sum is 0
+    // A thread holds 16 (last 32 columns of 96: 8) neighbouring columns of its rows.  Pieces of four columns change places
+    // within groups of four, by row and place, so that a store meets no bank twice.
+    const float f_ab[2] = {exp2_fast(ma - m_all[0]), exp2_fast(mb - m_all[1])};     // of no meaning where the sum is 0
+    auto place = [](int r, int f) { return f ^ ((f >> 3) & 1) ^ ((r & 1) << 1); };
 #pragma unroll
-    for (int t = 0; t < TILES; ++t) {
-        const int per = t < D / 64 * 8 ? 8 : 4, base = t < D / 64 * 8 ? t / 8 * 64 : D / 64 * 64, e = t < D / 64 * 8 ? t % 8 : t - D / 64 * 8;
-        const int col = base + 2 * c * per + e;
-        float* row = s_o + (warp * AT_ROWS + g) * D + col;
-        row[0] = la == 0.0f ? 0.0f : o[t][0] * fa;
-        row[per] = la == 0.0f ? 0.0f : o[t][1] * fa;
-        row += 8 * D;
-        row[0] = lb == 0.0f ? 0.0f : o[t][2] * fb;
-        row[per] = lb == 0.0f ? 0.0f : o[t][3] * fb;
+    for (int half = 0; half < 2; ++half) {
+        if ((half ? rb : ra) >= p.rows || (half ? lb : la) == 0.0f) continue;
+        const int r = g + 8 * half;
+        float4* row = reinterpret_cast<float4*>(s_o + (warp * AT_ROWS + r) * D);
+        const float f = f_ab[half];
+#pragma unroll
+        for (int t = 0; t < TILES; t += 4) {
+            const bool whole = t < D / 64 * 8;
+            const int at0 = whole ? t / 8 * 16 + 4 * c + t % 8 / 4 : D / 64 * 16 + 2 * c, step = whole ? 2 : 1;
+            row[place(r, at0)] = make_float4(o[t][2 * half] * f, o[t + 1][2 * half] * f, o[t + 2][2 * half] * f, o[t + 3][2 * half] * f);
+            row[place(r, at0 + step)] = make_float4(o[t][2 * half + 1] * f, o[t + 1][2 * half + 1] * f, o[t + 2][2 * half + 1] * f, o[t + 3][2 * half + 1] * f);
+        }
     }
     __syncthreads();
     const int rows = min(AT_ROWS, p.rows - r0);
@@ -317,21 +326,23 @@ __global__ void __launch_bounds__(AS_WARPS * 32, 2) attn_stream_kernel(const Att
         const int r = i / (D / 4), d = i % (D / 4) * 4;
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         float m = -INFINITY, l = 0.0f;
+        float2 ml[AS_WARPS];
 #pragma unroll
         for (int k = 0; k < AS_WARPS; ++k) {
-            const float4 x = *reinterpret_cast<const float4*>(s_o + (k * AT_ROWS + r) * D + d);
-            v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
-            m = fmaxf(m, s_ml[k * AT_ROWS + r].x);
+            ml[k] = s_ml[k * AT_ROWS + r];
+            m = fmaxf(m, ml[k].x);
         }
 #pragma unroll
         for (int k = 0; k < AS_WARPS; ++k) {
-            const float2 ml = s_ml[k * AT_ROWS + r];
-            if (ml.y != 0.0f) l += ml.y * exp2_fast(ml.x - m);
+            if (ml[k].y == 0.0f) continue;                         // that warp saw nothing and wrote nothing
+            const float4 x = reinterpret_cast<const float4*>(s_o + (k * AT_ROWS + r) * D)[place(r, d >> 2)];
+            v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+            l += ml[k].y * exp2_fast(ml[k].x - m);
         }
         const int64_t row = attn_row_index(p, b, h, r0 + r);
         if (p.part_ml != nullptr && d == 0) p.part_ml[row * p.nsplit + split] = make_float2(m, l);
         if (p.nsplit > 1) {
-            if (first < last) *reinterpret_cast<float4*>(p.part_o + (row * p.nsplit + split) * D + d) = v;
+            *reinterpret_cast<float4*>(p.part_o + (row * p.nsplit + split) * D + d) = v;
         } else {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             T* out = attn_out_row<T>(p, b, h, r0 + r) + d;
