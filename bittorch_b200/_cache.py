@@ -8,6 +8,7 @@ linear layers alone needs none of them.  Shapes and types are checked before dev
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import Optional, Sequence, Tuple
 
@@ -95,13 +96,13 @@ def _plain_memory(t: Tensor) -> bool:
     return True
 
 
-def _call(dev: torch.device, fn, *args) -> None:
-    """Enqueue on the current stream of ``dev``."""
-    if dev.index == torch.cuda.current_device():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+def _call(index: int, fn, *args) -> None:
+    """Enqueue on the current stream of device ``index``."""
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _C._check(rc)
 
@@ -126,8 +127,27 @@ def _cache_pair(what: str, k: Tensor, v: Tensor) -> None:
         _fail(f"{what}: the head dimension of a cache must be contiguous")
 
 
-def tree_attention(q: Tensor, k: Tensor, v: Tensor, lengths: Tensor, tree: Optional[Tensor], scale: Optional[float],
-                   mass: Optional[Tensor], out: Optional[Tensor]) -> Tensor:
+def _same_device(what: str, first: Tensor, *rest: Optional[Tensor]) -> int:
+    """The CUDA device index that all tensors are on."""
+    index = first.get_device()                         # -1: not on a device
+    for t in rest:
+        if t is not None and t.get_device() != index:
+            _on_one_device(what, first, *rest)
+    if index < 0 or not first.is_cuda:
+        _fail("All tensors must be CUDA")
+    return index
+
+
+def _sig(t: Optional[Tensor]):
+    """What the checks of a call go by: a call whose tensors have been seen with these is not checked again."""
+    return None if t is None else (t.shape, t.stride(), t.dtype)
+
+
+@functools.lru_cache(maxsize=1024)
+def _attention_plan(q_sig, k_sig, v_sig, len_sig, tree_sig, scale, mass_sig, out_sig, index):
+    """Checks the arguments of tree_attention; -> (what the C call takes of shapes and strides, workspace bytes)."""
+    q, k, v, lengths, tree, mass, out = (None if x is None else torch.empty_strided(x[0], x[1], dtype=x[2], device="meta")
+                                         for x in (q_sig, k_sig, v_sig, len_sig, tree_sig, mass_sig, out_sig))
     if q.dim() != 4:
         _fail("q must be 4D [B, H, T, D]")
     b, h, t, d = q.shape
@@ -151,9 +171,7 @@ def tree_attention(q: Tensor, k: Tensor, v: Tensor, lengths: Tensor, tree: Optio
         if tree.dtype is not torch.bool or tuple(tree.shape) not in ((t, t), (b, t, t)):
             _fail(f"tree must be bool [{t}, {t}] or [{b}, {t}, {t}], got {tree.dtype} {list(tree.shape)}")
         tree_sb = t * t if tree.dim() == 3 else 0
-    if scale is None:
-        scale = 1.0 / math.sqrt(d)
-    elif not math.isfinite(scale):
+    if not math.isfinite(scale):
         _fail("scale must be finite")
     if mass is not None:
         if mass.dtype is not torch.float32 or mass.shape != k.shape[:3]:
@@ -165,66 +183,81 @@ def tree_attention(q: Tensor, k: Tensor, v: Tensor, lengths: Tensor, tree: Optio
             _fail(f"out must be {q.dtype} {list(q.shape)}, got {out.dtype} {list(out.shape)}")
         if (out.stride(3) != 1 and d != 1) or not _plain_memory(out):
             _fail("out must have a contiguous head dimension and share no memory with itself")
-    _no_gradient("tree_attention", q, k, v, mass, out)
-    dev = _on_one_device("tree_attention", q, k, v, lengths, tree, mass, out)
+    if index < 0:
+        return None
+    out_strides = (t * h * d, d, h * d, 1) if out is None else out.stride()      # [B, T, H * D]: as the next projection reads it
+    q_strides = q.stride()[:3] if q.stride(3) == 1 or d == 1 else q.contiguous().stride()[:3]
+    strides = _TWELVE(*q_strides, *k.stride()[:3], *v.stride()[:3], *out_strides[:3])
+    code = _DT[q.dtype]
+    sizes = (b, h, hkv, t, s, d)
+    with torch.cuda.device(index):                     # the workspace depends on the device's SM count
+        need = _tree_attention_workspace(*sizes, code, mass is not None)
+    return (code, *sizes, strides), (len64, len_stride), tree_sb, ((0, 0) if mass is None else mass.stride()[:2]), need, out_strides
+
+
+def tree_attention(q: Tensor, k: Tensor, v: Tensor, lengths: Tensor, tree: Optional[Tensor], scale: Optional[float],
+                   mass: Optional[Tensor], out: Optional[Tensor]) -> Tensor:
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    plan = _attention_plan(_sig(q), _sig(k), _sig(v), _sig(lengths), _sig(tree), scale, _sig(mass), _sig(out), q.get_device())
+    if torch.is_grad_enabled():
+        _no_gradient("tree_attention", q, k, v, mass, out)
+    index = _same_device("tree_attention", q, k, v, lengths, tree, mass, out)
+    head, lens, tree_sb, mass_strides, need, out_strides = plan
     if q.stride(3) != 1:
         q = q.contiguous()
     if tree is not None and not tree.is_contiguous():
         tree = tree.contiguous()
-    if out is None:                       # the layout of the projection that follows: [B, T, H * D]
-        out = torch.empty((b, t, h, d), dtype=q.dtype, device=dev).transpose(1, 2)
-    code = _DT[q.dtype]
-    need = _workspace_bytes(dev, b, h, hkv, t, s, d, code, mass is not None)
+    dev = q.device
+    if out is None:
+        out = torch.empty_strided(q.shape, out_strides, dtype=q.dtype, device=dev)
     work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    strides = _TWELVE(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3])
-    mass_sb, mass_sh = (0, 0) if mass is None else mass.stride()[:2]
-    _call(dev, _tree_attention, q.data_ptr(), k.data_ptr(), v.data_ptr(), code, b, h, hkv, t, s, d, strides,
-          lengths.data_ptr(), len64, len_stride, None if tree is None else tree.data_ptr(), tree_sb, scale,
-          None if mass is None else mass.data_ptr(), mass_sb, mass_sh, out.data_ptr(),
-          None if work is None else work.data_ptr(), need)
+    _call(index, _tree_attention, q.data_ptr(), k.data_ptr(), v.data_ptr(), *head, lengths.data_ptr(), *lens,
+          None if tree is None else tree.data_ptr(), tree_sb, scale, None if mass is None else mass.data_ptr(), *mass_strides,
+          out.data_ptr(), None if work is None else work.data_ptr(), need)
     return out
 
 
-def _workspace_bytes(dev: torch.device, *sizes) -> int:
-    if dev.index == torch.cuda.current_device():       # it depends on the device's SM count
-        return _tree_attention_workspace(*sizes)
-    with torch.cuda.device(dev):
-        return _tree_attention_workspace(*sizes)
-
-
-def evict_select(mass: Tensor, lengths: Tensor, budget: int, sinks: int, recent: int) -> Tuple[Tensor, Tensor]:
+@functools.lru_cache(maxsize=1024)
+def _evict_plan(mass_sig, len_sig, budget, sinks, recent):
+    mass, lengths = (torch.empty_strided(x[0], x[1], dtype=x[2], device="meta") for x in (mass_sig, len_sig))
     if mass.dim() != 3 or mass.dtype is not torch.float32 or mass.numel() == 0:
         _fail(f"mass must be float32 [B, Hkv, S], got {mass.dtype} {list(mass.shape)}")
     if mass.stride(2) != 1 and mass.shape[2] != 1:
         _fail("mass must have contiguous slots")
     b, hkv, s = mass.shape
-    budget, sinks, recent = int(budget), int(sinks), int(recent)
     if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
         _fail(f"a budget of {budget} slots must be positive and hold {sinks} sinks and {recent} recent slots")
-    len64, len_stride = _lengths(lengths, b)
-    dev = _on_one_device("evict_select", mass, lengths)
-    keep = torch.empty((b, hkv, budget), dtype=torch.int64, device=dev)
-    counts = torch.empty((b,), dtype=torch.int64, device=dev)
-    _call(dev, _evict_select, mass.data_ptr(), mass.stride(0), mass.stride(1), b, hkv, s, lengths.data_ptr(), len64, len_stride,
-          budget, sinks, recent, keep.data_ptr(), counts.data_ptr())
+    return (b, hkv, s), mass.stride()[:2], _lengths(lengths, b)
+
+
+def evict_select(mass: Tensor, lengths: Tensor, budget: int, sinks: int, recent: int) -> Tuple[Tensor, Tensor]:
+    budget, sinks, recent = int(budget), int(sinks), int(recent)
+    sizes, strides, lens = _evict_plan(_sig(mass), _sig(lengths), budget, sinks, recent)
+    index = _same_device("evict_select", mass, lengths)
+    b, hkv, _ = sizes
+    keep = torch.empty((b, hkv, budget), dtype=torch.int64, device=mass.device)
+    counts = torch.empty((b,), dtype=torch.int64, device=mass.device)
+    _call(index, _evict_select, mass.data_ptr(), *strides, *sizes, lengths.data_ptr(), *lens, budget, sinks, recent, keep.data_ptr(),
+          counts.data_ptr())
     return keep, counts
 
 
-def compact_cache(k: Tensor, v: Tensor, keep: Tensor, counts: Tensor, first: Optional[Tensor], mass: Optional[Tensor],
-                  out: Optional[Sequence[Tensor]]) -> None:
+@functools.lru_cache(maxsize=1024)
+def _compact_plan(k_sig, v_sig, keep_sig, counts_sig, first_sig, mass_sig, out_sigs):
+    make = lambda x: None if x is None else torch.empty_strided(x[0], x[1], dtype=x[2], device="meta")
+    k, v, keep, counts, first, mass = (make(x) for x in (k_sig, v_sig, keep_sig, counts_sig, first_sig, mass_sig))
     _cache_pair("compact_cache", k, v)
     b, hkv, s, d = k.shape
-    if out is None:
+    if out_sigs is None:
         k_out, v_out, mass_out = k, v, mass
     else:
-        if len(out) != (2 if mass is None else 3):
+        if len(out_sigs) != (2 if mass is None else 3):
             _fail("out must be (keys, values), with the mass third where one is given")
-        k_out, v_out, mass_out = out[0], out[1], (out[2] if mass is not None else None)
+        k_out, v_out, mass_out = make(out_sigs[0]), make(out_sigs[1]), (make(out_sigs[2]) if mass is not None else None)
         _cache_pair("compact_cache", k_out, v_out)
         if k_out.dtype != k.dtype or k_out.shape[:2] != k.shape[:2] or k_out.shape[3] != d:
             _fail(f"out must be {k.dtype} [{b}, {hkv}, slots, {d}], got {k_out.dtype} {list(k_out.shape)}")
-        if k_out.data_ptr() in (k.data_ptr(), v.data_ptr()) or v_out.data_ptr() in (k.data_ptr(), v.data_ptr(), k_out.data_ptr()):
-            _fail("out must be other memory than the cache (leave it out to compact in place)")
     s_out = k_out.shape[2]
     if keep.dim() != 3 or keep.dtype is not torch.int64 or keep.shape[0] != b or keep.shape[1] not in (1, hkv) or keep.shape[2] == 0:
         _fail(f"keep must be int64 [{b}, {hkv} or 1, n], got {keep.dtype} {list(keep.shape)}")
@@ -235,26 +268,40 @@ def compact_cache(k: Tensor, v: Tensor, keep: Tensor, counts: Tensor, first: Opt
         for m, slots in ((mass, s), (mass_out, s_out)):
             if m.dtype is not torch.float32 or tuple(m.shape) != (b, hkv, slots) or (m.stride(2) != 1 and slots != 1):
                 _fail(f"mass must be float32 [{b}, {hkv}, {slots}] with contiguous slots, got {m.dtype} {list(m.shape)}")
-        if out is not None and mass_out.data_ptr() == mass.data_ptr():
-            _fail("out must be other memory than the mass (leave it out to compact in place)")
     if not (_plain_memory(k_out) and _plain_memory(v_out) and (mass_out is None or _plain_memory(mass_out))):
         _fail("compact_cache: what is written must share no memory with itself")
-    _no_gradient("compact_cache", k, v, k_out, v_out, mass, mass_out)
-    dev = _on_one_device("compact_cache", k, v, k_out, v_out, keep, counts, first, mass, mass_out)
+    n = keep.shape[2]
+    keep_strides = keep.stride() if keep.stride(2) == 1 or n == 1 else keep.contiguous().stride()
+    strides = _TWELVE(*k.stride()[:3], *v.stride()[:3], *k_out.stride()[:3], *v_out.stride()[:3])
+    mass_strides = None if mass is None else _FOUR(*mass.stride()[:2], *mass_out.stride()[:2])
+    return (_DT[k.dtype], b, hkv, s, s_out, d, strides), (keep_strides[0], keep_strides[1] if keep.shape[1] == hkv else 0, n), mass_strides
+
+
+def compact_cache(k: Tensor, v: Tensor, keep: Tensor, counts: Tensor, first: Optional[Tensor], mass: Optional[Tensor],
+                  out: Optional[Sequence[Tensor]]) -> None:
+    head, tail, mass_strides = _compact_plan(_sig(k), _sig(v), _sig(keep), _sig(counts), _sig(first), _sig(mass),
+                                             None if out is None else tuple(_sig(x) for x in out))
+    k_out, v_out, mass_out = (k, v, mass) if out is None else (out[0], out[1], out[2] if mass is not None else None)
+    if torch.is_grad_enabled():
+        _no_gradient("compact_cache", k, v, k_out, v_out, mass, mass_out)
+    if out is not None:
+        apart = [x.data_ptr() for x in (k, v, k_out, v_out)]
+        if apart[2] in apart[:2] or apart[3] in apart[:3] or (mass is not None and mass_out.data_ptr() == mass.data_ptr()):
+            _fail("out must be other memory than the cache (leave it out to compact in place)")
+    index = _same_device("compact_cache", k, v, k_out, v_out, keep, counts, first, mass, mass_out)
     if keep.stride(2) != 1:
         keep = keep.contiguous()
     counts = counts.contiguous()
     first = None if first is None else first.contiguous()
-    strides = _TWELVE(*k.stride()[:3], *v.stride()[:3], *k_out.stride()[:3], *v_out.stride()[:3])
-    mass_strides = None if mass is None else _FOUR(*mass.stride()[:2], *mass_out.stride()[:2])
-    _call(dev, _compact_cache, k.data_ptr(), v.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), _DT[k.dtype], b, hkv, s, s_out, d,
-          strides, keep.data_ptr(), keep.stride(0), keep.stride(1) if keep.shape[1] == hkv else 0, keep.shape[2],
+    _call(index, _compact_cache, k.data_ptr(), v.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), *head, keep.data_ptr(), *tail,
           counts.data_ptr(), None if first is None else first.data_ptr(), None if mass is None else mass.data_ptr(),
           None if mass is None else mass_out.data_ptr(), mass_strides)
 
 
-def beam_select(logits: Tensor, scores: Tensor, select: Optional[int], finished: Optional[Tensor],
-                end_token: Optional[int]) -> Tuple[Tensor, Tensor, Tensor]:
+@functools.lru_cache(maxsize=1024)
+def _beam_plan(logits_sig, scores_sig, select, finished_sig, end_token):
+    logits, scores, finished = (None if x is None else torch.empty_strided(x[0], x[1], dtype=x[2], device="meta")
+                                for x in (logits_sig, scores_sig, finished_sig))
     if logits.dim() != 3 or logits.dtype not in _DT:
         _fail(f"logits must be float32, float16 or bfloat16 [B, beams, vocabulary], got {logits.dtype} {list(logits.shape)}")
     b, w, vocab = logits.shape
@@ -274,61 +321,73 @@ def beam_select(logits: Tensor, scores: Tensor, select: Optional[int], finished:
             _fail(f"finished must be bool [{b}, {w}], got {finished.dtype} {list(finished.shape)}")
         if not 0 <= end_token < vocab:
             _fail(f"end_token {end_token} is outside the vocabulary of {vocab}")
-    _no_gradient("beam_select", logits, scores)
-    dev = _on_one_device("beam_select", logits, scores, finished)
+    code = _DT[logits.dtype]
+    strides = logits.stride()[:2] if logits.stride(2) == 1 or vocab == 1 else logits.contiguous().stride()[:2]
+    return (code, b, w, vocab, *strides), n, _beam_select_workspace(b, w, vocab, code, n)
+
+
+def beam_select(logits: Tensor, scores: Tensor, select: Optional[int], finished: Optional[Tensor],
+                end_token: Optional[int]) -> Tuple[Tensor, Tensor, Tensor]:
+    head, n, need = _beam_plan(_sig(logits), _sig(scores), select, _sig(finished), end_token)
+    if torch.is_grad_enabled():
+        _no_gradient("beam_select", logits, scores)
+    index = _same_device("beam_select", logits, scores, finished)
     if logits.stride(2) != 1:
         logits = logits.contiguous()
-    scores = scores.contiguous()
-    finished = None if finished is None else finished.contiguous()
-    code = _DT[logits.dtype]
-    need = _beam_select_workspace(b, w, vocab, code, n)
+    if not scores.is_contiguous():
+        scores = scores.contiguous()
+    if finished is not None and not finished.is_contiguous():
+        finished = finished.contiguous()
+    dev, b = logits.device, head[1]
     out = torch.empty((b, n), dtype=torch.float32, device=dev)
-    picks = torch.empty((2, b, n), dtype=torch.int64, device=dev)
+    tokens, parents = torch.empty((2, b, n), dtype=torch.int64, device=dev).unbind()
     work = torch.empty(need, dtype=torch.uint8, device=dev)
-    tokens, parents = picks[0], picks[1]
-    _call(dev, _beam_select, logits.data_ptr(), code, b, w, vocab, logits.stride(0), logits.stride(1), scores.data_ptr(),
-          None if finished is None else finished.data_ptr(), 0 if end_token is None else int(end_token), n, out.data_ptr(),
-          tokens.data_ptr(), parents.data_ptr(), work.data_ptr(), need)
+    _call(index, _beam_select, logits.data_ptr(), *head, scores.data_ptr(), None if finished is None else finished.data_ptr(),
+          0 if end_token is None else end_token, n, out.data_ptr(), tokens.data_ptr(), parents.data_ptr(), work.data_ptr(), need)
     return out, tokens, parents
 
 
-def reorder_cache(caches: Sequence[Tensor], parents: Tensor, lengths: Tensor, start: int) -> None:
-    if len(caches) == 0:
+@functools.lru_cache(maxsize=1024)
+def _reorder_plan(sigs, parents_sig, len_sig, start):
+    parents, lengths = (torch.empty_strided(x[0], x[1], dtype=x[2], device="meta") for x in (parents_sig, len_sig))
+    if len(sigs) == 0:
         _fail("reorder_cache: no cache tensors")
     if parents.dim() != 2 or parents.dtype is not torch.int64 or parents.numel() == 0:
         _fail(f"parents must be int64 [B, beams], got {parents.dtype} {list(parents.shape)}")
     b, w = parents.shape
     if w > REORDER_MAX_BEAMS:
         _fail(f"up to {REORDER_MAX_BEAMS} beams are supported, got {w}")
-    shape, dtype = caches[0].shape, caches[0].dtype
-    if len(shape) != 4 or shape[0] != b * w or caches[0].numel() == 0 or dtype not in _DT:
+    shape, _, dtype = sigs[0]
+    if len(shape) != 4 or shape[0] != b * w or 0 in shape or dtype not in _DT:
         _fail(f"cache tensors must be float32, float16 or bfloat16 [{b * w}, Hkv, S, D], got {dtype} {list(shape)}")
-    start = int(start)
     _require(start >= 0, "start must not be negative")
-    len64, len_stride = _lengths(lengths, b)
-    dev = parents.device
-    pointers, strides = [], []
-    contiguous = True
-    grad = torch.is_grad_enabled()
-    for c in caches:
-        if c.shape != shape or c.dtype != dtype:
+    strides, spans = [], []
+    for size, stride, kind in sigs:
+        if size != shape or kind != dtype:
             _fail("reorder_cache: all cache tensors must have one shape and type")
-        st = c.stride()
-        if not c.is_contiguous():
-            contiguous = False
-            if (st[3] != 1 and shape[3] != 1) or not _plain_memory(c):
-                _fail("reorder_cache: cache tensors must have a contiguous head dimension and share no memory with themselves")
-        if grad and c.requires_grad:
-            _no_gradient("reorder_cache", c)
-        pointers.append(c.data_ptr())
-        strides += st[:3]
-    _on_one_device("reorder_cache", parents, lengths, *caches)
-    if len(set(pointers)) < len(pointers):
-        _fail("reorder_cache: a cache tensor is listed twice")
-    if contiguous and len(pointers) > 1:
-        ordered, size = sorted(pointers), caches[0].numel() * caches[0].element_size()
-        _require(all(y - x >= size for x, y in zip(ordered, ordered[1:])), "reorder_cache: cache tensors share memory")
-    parents = parents.contiguous()
-    count = len(pointers)
-    _call(dev, _reorder_cache, (_p * count)(*pointers), count, _DT[dtype], b, w, shape[1], shape[2], shape[3],
-          (_i64 * (3 * count))(*strides), parents.data_ptr(), lengths.data_ptr(), len64, len_stride, start)
+        if (stride[3] != 1 and shape[3] != 1) or not _plain_memory(torch.empty_strided(size, stride, dtype=kind, device="meta")):
+            _fail("reorder_cache: cache tensors must have a contiguous head dimension and share no memory with themselves")
+        strides += stride[:3]
+        spans.append(1 + sum((n - 1) * st for n, st in zip(size, stride)))
+    bytes_each = torch.empty(0, dtype=dtype).element_size()
+    count = len(sigs)
+    return ((count, _DT[dtype], b, w, *shape[1:], (_i64 * (3 * count))(*strides)), _lengths(lengths, b),
+            tuple(n * bytes_each for n in spans), _p * count)
+
+
+def reorder_cache(caches: Sequence[Tensor], parents: Tensor, lengths: Tensor, start: int) -> None:
+    start = int(start)
+    head, lens, spans, pointer_array = _reorder_plan(tuple([_sig(c) for c in caches]), _sig(parents), _sig(lengths), start)
+    if torch.is_grad_enabled():
+        _no_gradient("reorder_cache", *caches)
+    index = _same_device("reorder_cache", parents, lengths, *caches)
+    pointers = [c.data_ptr() for c in caches]
+    if len(pointers) > 1:
+        # tensors of one shape that interleave in memory (views of one buffer) are told apart by their first elements alone
+        ordered = sorted(zip(pointers, spans, caches), key=lambda x: x[0])
+        for (p0, n0, c0), (p1, _, c1) in zip(ordered, ordered[1:]):
+            if p1 == p0 or (p1 - p0 < n0 and c0.is_contiguous() and c1.is_contiguous()):
+                _fail("reorder_cache: a cache tensor is listed twice, or two share memory")
+    if not parents.is_contiguous():
+        parents = parents.contiguous()
+    _call(index, _reorder_cache, pointer_array(*pointers), *head, parents.data_ptr(), lengths.data_ptr(), *lens, start)

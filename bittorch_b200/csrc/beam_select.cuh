@@ -4,13 +4,15 @@
 // one piece of a row, held in registers, and leaves the piece's maximum, its sum of exponentials and its n largest
 // logits; beam_join makes the log-sums and ranks the survivors of all beams in float64.  Bound by HBM (the logits).
 //
-// The n largest of a piece: a logit and its place make one 64-bit key (larger logit first, then the lower place), so no
-// two are equal.  Every thread's largest key is compared with all others; the n-th of those bounds the n-th of the
-// piece from below, and only the n threads above it can hold more: at most n x 32 keys are collected and ranked by
-// counting, usually little more than n.
+// The n largest of a piece: 64 groups of four threads have a maximum each, and the n-th of those (n <= 64) bounds the
+// n-th of the piece from below.  What is not below it is collected and ranked by counting: with independent logits a
+// little more than n.  A logit and its place make one 64-bit key (larger logit first, then the lower place), so that no
+// two are equal.  A plateau of equal logits can pass the bound in any number; a list that overflows is abandoned for n
+// searches of the largest key below the last.
 //
 // A row's elements go to threads by their place in the row, whatever the row's alignment (a misaligned row is read in
-// aligned 16-byte words and shifted): equal rows have equal sums, so that ties between beams are ties.
+// aligned 16-byte words and shifted): equal rows have equal sums, so that ties between beams are ties.  Exponentials
+// are float32 (2^-22), their sums float32 within a thread (32 terms) and float64 from there.
 #pragma once
 
 #include "cache_common.cuh"
@@ -19,10 +21,14 @@
 namespace bt {
 
 constexpr int BS_THREADS = 256;
+constexpr int BS_WARPS = BS_THREADS / 32;
 constexpr int BS_WORDS = 4;                                        // 16-byte words of a thread
+constexpr int BS_GROUPS = BS_THREADS / 4;                          // at least BT_BEAM_MAX_SELECT
+constexpr int BS_LIST = 1024;
+static_assert(BS_GROUPS >= BT_BEAM_MAX_SELECT, "the n-th group maximum must exist");
 template <typename T> __host__ __device__ constexpr int bs_per_word() { return 16 / static_cast<int>(sizeof(T)); }
 template <typename T> __host__ __device__ constexpr int bs_piece() { return BS_THREADS * BS_WORDS * bs_per_word<T>(); }
-constexpr int BJ_LIST = 2048;                                      // candidates that beam_join ranks by counting
+constexpr int BJ_LIST = 1024;                                      // candidates that beam_join ranks by counting
 
 struct BeamParams {
     const void* logits;
@@ -97,99 +103,224 @@ __device__ __forceinline__ void widen_word<__half>(uint4 w, float* x) {
         x[2 * i + 1] = __high2float(h);
     }
 }
+// Largest element of a word so far; a NaN is dropped.  16-bit types: two at a time, `acc` holds the even and odd places.
+template <typename T> struct WordMax;
+template <> struct WordMax<float> {
+    float m = -INFINITY;
+    __device__ __forceinline__ void add(uint4 w) {
+        m = fmaxf(fmaxf(m, __uint_as_float(w.x)), fmaxf(__uint_as_float(w.y), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w))));
+    }
+    __device__ __forceinline__ float get() const { return m; }
+};
+#ifdef BT_SIMT_HOST
+template <typename T> struct WordMax {
+    float m = -INFINITY;
+    void add(uint4 w) {
+        float x[8];
+        widen_word<T>(w, x);
+        for (int e = 0; e < 8; ++e) m = fmaxf(m, x[e]);
+    }
+    float get() const { return m; }
+};
+#else
+template <> struct WordMax<__nv_bfloat16> {
+    __nv_bfloat162 m = __float2bfloat162_rn(-INFINITY);
+    __device__ __forceinline__ void add(uint4 w) {
+        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
+        m = __hmax2(__hmax2(m, h[0]), __hmax2(__hmax2(h[1], h[2]), h[3]));
+    }
+    __device__ __forceinline__ float get() const { return fmaxf(__low2float(m), __high2float(m)); }
+};
+template <> struct WordMax<__half> {
+    __half2 m = __float2half2_rn(-INFINITY);
+    __device__ __forceinline__ void add(uint4 w) {
+        const __half2* h = reinterpret_cast<const __half2*>(&w);
+        m = __hmax2(__hmax2(m, h[0]), __hmax2(__hmax2(h[1], h[2]), h[3]));
+    }
+    __device__ __forceinline__ float get() const { return fmaxf(__low2float(m), __high2float(m)); }
+};
+#endif
+// A word of which elements [0, valid) come from memory and the rest are -infinity
+template <typename T>
+__device__ __forceinline__ uint4 partial_word(const T* x, int64_t valid) {
+    union { T e[bs_per_word<T>()]; uint4 w; } u;
+    for (int i = 0; i < bs_per_word<T>(); ++i) u.e[i] = i < valid ? x[i] : from_float<T>(-INFINITY);
+    return u.w;
+}
+// Words as the row has them, whatever its alignment: word `wi` is elements [wi * PER, +PER).  This form for the row's ends.
+template <typename T>
+__device__ __noinline__ uint4 row_word_at_end(const T* x0, int64_t V, int64_t wi) {
+    const int64_t v = wi * bs_per_word<T>();
+    return v < V ? partial_word<T>(x0 + v, V - v) : partial_word<T>(x0, 0);
+}
+// Makes the compiler forget what it derived from the word: keeping 32 widened values instead of 16 packed ones would
+// halve the warps of an SM.
+__device__ __forceinline__ void keep_packed(uint4& w) {
+#ifndef BT_SIMT_HOST
+    asm volatile("" : "+r"(w.x), "+r"(w.y), "+r"(w.z), "+r"(w.w));
+#endif
+}
+__device__ __forceinline__ unsigned long long logit_key(float x, int64_t v) {
+    return (static_cast<unsigned long long>(ordered_key(x != x ? -INFINITY : x)) << 32) | (0xffffffffu - static_cast<uint32_t>(v));
+}
 
 template <typename T>
-__global__ void __launch_bounds__(BS_THREADS) beam_scan_kernel(const BeamParams p) {
-    constexpr int PER = bs_per_word<T>(), E = BS_WORDS * PER, PIECE = bs_piece<T>();
-    __shared__ unsigned long long s_best[BS_THREADS];
-    __shared__ unsigned long long s_list[BT_BEAM_MAX_SELECT * E];
-    __shared__ double s_sum[BS_THREADS / 32];
-    __shared__ float s_max[BS_THREADS / 32];
-    __shared__ unsigned long long s_edge;
+__global__ void __launch_bounds__(BS_THREADS, 8) beam_scan_kernel(const BeamParams p) {
+    constexpr int PER = bs_per_word<T>(), PIECE = bs_piece<T>();
+    __shared__ unsigned long long s_list[BS_LIST];
+    __shared__ double s_sum[BS_WARPS];
+    __shared__ float s_max[BS_WARPS], s_group[BS_GROUPS];
+    __shared__ unsigned long long s_best[BS_WARPS];
+    __shared__ float s_edge;
     __shared__ int s_count;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int64_t row = blockIdx.x / p.pieces;
-    const int piece = static_cast<int>(blockIdx.x % p.pieces);
-    if (tid == 0) s_count = 0, s_edge = 0;
+    const int64_t row = blockIdx.x / static_cast<unsigned>(p.pieces);
+    const int piece = static_cast<int>(blockIdx.x - static_cast<unsigned>(row) * p.pieces);
+    if (tid == 0) s_count = 0;
     pdl_launch_dependents();
     pdl_wait();
     if (!beam_live(p, row)) return;                                // for every thread of the CTA; beam_join knows
-    const T* x0 = static_cast<const T*>(p.logits) + row / p.W * p.ld_b + row % p.W * p.ld_w;
+    const int64_t b = row / p.W;
+    const T* x0 = static_cast<const T*>(p.logits) + b * p.ld_b + (row - b * p.W) * p.ld_w;
+    const int64_t v0 = static_cast<int64_t>(piece) * PIECE;
+    const int64_t w0 = v0 / PER + tid;                             // this thread's first word; the others follow at BS_THREADS
+
     const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(x0) & 15);
     const uint4* words = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(x0) - shift);
-    const int64_t v0 = static_cast<int64_t>(piece) * PIECE;
-
-    float x[E];
-    unsigned long long best = 0;
-    float mx = -INFINITY;
+    uint4 word[BS_WORDS];
 #pragma unroll
     for (int i = 0; i < BS_WORDS; ++i) {
-        const int64_t v = v0 + (static_cast<int64_t>(i) * BS_THREADS + tid) * PER;     // first element of the word
-        const int64_t wi = v / PER;
-        if (v + PER <= p.V && (shift == 0 || (wi > 0 && v + 2 * PER <= p.V))) {         // all bytes read lie in the row
-            const uint4 lo = words[wi];
-            widen_word<T>(shift == 0 ? lo : shifted_word(lo, words[wi + 1], shift), x + i * PER);
-        } else {
-#pragma unroll
-            for (int e = 0; e < PER; ++e) x[i * PER + e] = v + e < p.V ? to_float<T>(x0[v + e]) : -INFINITY;
-        }
-#pragma unroll
-        for (int e = 0; e < PER; ++e) {
-            float& f = x[i * PER + e];
-            if (f != f) f = -INFINITY;                             // a NaN is never better than a number
-            mx = fmaxf(mx, f);
-            if (v + e < p.V) {
-                const unsigned long long key = (static_cast<unsigned long long>(ordered_key(f)) << 32) | (0xffffffffu - static_cast<uint32_t>(v + e));
-                if (key > best) best = key;
-            }
-        }
+        const int64_t wi = w0 + i * BS_THREADS;
+        // a shifted word takes bytes of two aligned ones, all of which have to lie in the row
+        if (shift == 0 && (wi + 1) * PER <= p.V) word[i] = words[wi];
+        else if (wi > 0 && (wi + 2) * PER <= p.V) word[i] = shifted_word(words[wi], words[wi + 1], shift);
+        else word[i] = row_word_at_end<T>(x0, p.V, wi);
     }
-    s_best[tid] = best;
-    mx = warp_max(mx);
-    if (lane == 0) s_max[warp] = mx;
-    __syncthreads();
-    mx = s_max[0];
+    WordMax<T> top;
 #pragma unroll
-    for (int i = 1; i < BS_THREADS / 32; ++i) mx = fmaxf(mx, s_max[i]);
+    for (int i = 0; i < BS_WORDS; ++i) top.add(word[i]);
+    const float mine = top.get();
+    float mx = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    if ((lane & 3) == 0) s_group[tid >> 2] = mx;
+    mx = warp_max(mx);
+    __syncthreads();
+    {   // the n-th largest group maximum: the four threads of a group count the others above it, 16 each
+        const float a = s_group[tid >> 2];
+        int above = 0, level = 0;
+#pragma unroll
+        for (int i = 0; i < BS_GROUPS / 4; ++i) {
+            const float x = s_group[(tid & 3) * (BS_GROUPS / 4) + i];
+            above += x > a;
+            level += x >= a;
+        }
+        above += __shfl_xor_sync(0xffffffffu, above, 1);
+        level += __shfl_xor_sync(0xffffffffu, level, 1);
+        above += __shfl_xor_sync(0xffffffffu, above, 2);
+        level += __shfl_xor_sync(0xffffffffu, level, 2);
+        if (above < p.n && level >= p.n) s_edge = a;               // groups that tie here write the same value
+    }
     float sum = 0.0f;
     if (mx - mx == 0.0f) {                                         // finite
 #pragma unroll
-        for (int e = 0; e < E; ++e) sum += expf(x[e] - mx);
+        for (int i = 0; i < BS_WORDS; ++i) {
+            float x[PER];
+            keep_packed(word[i]);
+            widen_word<T>(word[i], x);
+#pragma unroll
+            for (int e = 0; e < PER; ++e) sum += exp2_fast((fmaxf(x[e], -INFINITY) - mx) * 1.4426950408889634f);     // a NaN adds 0
+        }
     }
     const double total = warp_add_double(static_cast<double>(sum));
-    if (lane == 0) s_sum[warp] = total;
-    // the n-th largest of the threads' best keys
-    int above = 0;
-    for (int i = 0; i < BS_THREADS; ++i) above += s_best[i] > best;
-    if (above == p.n - 1 && best != 0) s_edge = best;
+    if (lane == 0) {
+        s_sum[warp] = total;
+        s_max[warp] = mx;
+    }
     __syncthreads();
-    const unsigned long long edge = s_edge;                        // 0: fewer than n threads hold anything
-    if (best >= edge && best != 0) {
+    const float edge = s_edge;
+    if (mine >= edge && mine > -INFINITY) {
 #pragma unroll
-        for (int i = 0; i < BS_WORDS; ++i)
+        for (int i = 0; i < BS_WORDS; ++i) {
+            keep_packed(word[i]);
+            WordMax<T> here;
+            here.add(word[i]);
+            if (!(here.get() >= edge)) continue;
+            float x[PER];
+            widen_word<T>(word[i], x);
 #pragma unroll
-            for (int e = 0; e < PER; ++e) {
-                const int64_t v = v0 + (static_cast<int64_t>(i) * BS_THREADS + tid) * PER + e;
-                const unsigned long long key = (static_cast<unsigned long long>(ordered_key(x[i * PER + e])) << 32) | (0xffffffffu - static_cast<uint32_t>(v));
-                if (v < p.V && key >= edge) s_list[atomicAdd(&s_count, 1)] = key;
-            }
+            for (int e = 0; e < PER; ++e)
+                if (x[e] >= edge && x[e] > -INFINITY) {
+                    const int at = atomicAdd(&s_count, 1);
+                    if (at < BS_LIST) s_list[at] = logit_key(x[e], (w0 + i * BS_THREADS) * PER + e);
+                }
+        }
     }
     __syncthreads();
     const int count = s_count;
     unsigned long long* out = p.keys + (row * p.pieces + piece) * p.n;
-    for (int i = tid; i < count; i += BS_THREADS) {
-        const unsigned long long key = s_list[i];
-        int rank = 0;
-        for (int j = 0; j < count; ++j) rank += s_list[j] > key;
-        if (rank < p.n) out[rank] = key;
-    }
-    for (int i = count + tid; i < p.n; i += BS_THREADS) out[i] = 0;
-    if (tid == 0) {
+    if (warp == 0) {                                               // the warps' sums become one, a lane per warp
+        const float m_w = lane < BS_WARPS ? s_max[lane] : -INFINITY, m = warp_max(m_w);
         double all = 0.0;
+        if (lane < BS_WARPS && m - m == 0.0f && s_sum[lane] > 0.0)
+            all = s_sum[lane] * exp2(1.4426950408889634 * (static_cast<double>(m_w) - static_cast<double>(m)));
+        all = warp_add_double(all);
+        if (lane == 0) {
+            p.piece_max[row * p.pieces + piece] = m;
+            p.piece_sum[row * p.pieces + piece] = all;
+        }
+    }
+    if (count <= BS_LIST) {
+        for (int i = tid; i < count; i += BS_THREADS) {
+            const unsigned long long key = s_list[i];
+            int rank = 0;
+            for (int j = 0; j < count; ++j) rank += s_list[j] > key;
+            if (rank < p.n) out[rank] = key;
+        }
+        // Fewer than n numbers above -infinity: the lowest places among the others come next, and as only `count` places
+        // hold a number, they are found among the first n.
+        if (count < p.n && warp == BS_WARPS - 1) {
+            int at = count;
+            for (int i0 = 0; i0 < p.n; i0 += 32) {
+                const int64_t v = v0 + i0 + lane;
+                const float x = i0 + lane < p.n && v < p.V ? to_float<T>(x0[v]) : 0.0f;
+                const bool low = !(x > -INFINITY);
+                const unsigned mask = __ballot_sync(0xffffffffu, low);
+                const int to = at + __popc(mask & ((1u << lane) - 1));
+                if (low && to < p.n) out[to] = logit_key(x, v);
+                at += __popc(mask);
+            }
+            for (int i = at + lane; i < p.n; i += 32) out[i] = 0;  // the row ends before that
+        }
+        return;
+    }
+    unsigned long long last = ~0ull;
+    for (int k = 0; k < p.n; ++k) {
+        unsigned long long best = 0;
 #pragma unroll
-        for (int i = 0; i < BS_THREADS / 32; ++i) all += s_sum[i];
-        p.piece_max[row * p.pieces + piece] = mx;
-        p.piece_sum[row * p.pieces + piece] = all;
+        for (int i = 0; i < BS_WORDS; ++i) {
+            float x[PER];
+            keep_packed(word[i]);
+            widen_word<T>(word[i], x);
+#pragma unroll
+            for (int e = 0; e < PER; ++e) {
+                const int64_t v = (w0 + i * BS_THREADS) * PER + e;
+                const unsigned long long key = v < p.V ? logit_key(x[e], v) : 0;
+                if (key < last && key > best) best = key;
+            }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const unsigned hi = __shfl_xor_sync(0xffffffffu, static_cast<unsigned>(best >> 32), o);
+            const unsigned lo = __shfl_xor_sync(0xffffffffu, static_cast<unsigned>(best), o);
+            const unsigned long long other = (static_cast<unsigned long long>(hi) << 32) | lo;
+            if (other > best) best = other;
+        }
+        if (lane == 0) s_best[warp] = best;
+        __syncthreads();
+        last = s_best[0];
+        for (int i = 1; i < BS_WARPS; ++i) last = s_best[i] > last ? s_best[i] : last;
+        if (tid == 0) out[k] = last;
+        __syncthreads();
     }
 }
 
@@ -202,13 +333,13 @@ struct Candidate {
     }
 };
 
-// Survivor `i` of a sequence: entry i % n of piece i / n % pieces of beam i / n / pieces
-__device__ __forceinline__ Candidate beam_candidate(const BeamParams& p, int b, int64_t i, const double* s_base, const uint8_t* s_kind) {
-    const int e = static_cast<int>(i % p.n), piece = static_cast<int>(i / p.n % p.pieces), w = static_cast<int>(i / p.n / p.pieces);
+// Entry e of the list that piece `piece` of beam w left
+__device__ __forceinline__ Candidate beam_candidate(const BeamParams& p, int64_t b, int w, int piece, int e, const double* s_base,
+                                                    const uint8_t* s_kind) {
     Candidate c = {-INFINITY, -1};
     int64_t token;
     if (s_kind[w] == 0) {                                          // live: what beam_scan left
-        const unsigned long long key = p.keys[((static_cast<int64_t>(b) * p.W + w) * p.pieces + piece) * p.n + e];
+        const unsigned long long key = p.keys[((b * p.W + w) * p.pieces + piece) * p.n + e];
         if (key == 0) return c;
         token = 0xffffffffu - static_cast<uint32_t>(key);
         c.score = s_base[w] + static_cast<double>(key_value(static_cast<uint32_t>(key >> 32)));
@@ -264,21 +395,28 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const BeamParams 
         }
     }
     __syncthreads();
-    const int64_t total = static_cast<int64_t>(p.W) * p.pieces * p.n;
+    // Lists are sorted, so a thread that owns some of them knows its best from their heads.  With at least n threads, the
+    // n-th best of those bounds the n-th best of all from below.
+    const unsigned lists = static_cast<unsigned>(p.W) * p.pieces;
     Candidate best = {-INFINITY, -1};
-    for (int64_t i = tid; i < total; i += BJ_THREADS) {
-        const Candidate c = beam_candidate(p, b, i, s_base, s_kind);
+    for (unsigned i = tid; i < lists; i += BJ_THREADS) {
+        const Candidate c = beam_candidate(p, b, i / p.pieces, i % p.pieces, 0, s_base, s_kind);
         if (c.better(best)) best = c;
     }
     s_best[tid] = best;
     __syncthreads();
-    int above = 0;
-    for (int i = 0; i < BJ_THREADS; ++i) above += s_best[i].better(best);
-    if (above == p.n - 1 && best.place >= 0) s_edge = best;
+    if (best.place >= 0) {
+        const int heads = lists < BJ_THREADS ? lists : BJ_THREADS;
+        int above = 0;
+        for (int i = 0; i < heads; ++i) above += s_best[i].better(best);
+        if (above == p.n - 1) s_edge = best;
+    }
     __syncthreads();
     const Candidate edge = s_edge;
-    for (int64_t i = tid; i < total; i += BJ_THREADS) {
-        const Candidate c = beam_candidate(p, b, i, s_base, s_kind);
+#pragma unroll 4
+    for (unsigned i = tid; i < lists * p.n; i += BJ_THREADS) {     // all entries: their loads do not wait for one another
+        const unsigned list = i / p.n, w = list / p.pieces;
+        const Candidate c = beam_candidate(p, b, w, list - w * p.pieces, i - list * p.n, s_base, s_kind);
         if (c.place < 0 || edge.better(c)) continue;
         const int at = atomicAdd(&s_count, 1);
         if (at < BJ_LIST) s_list[at] = c;
@@ -293,21 +431,26 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const BeamParams 
             for (int j = 0; j < count; ++j) rank += s_list[j].better(c);
             if (rank < p.n) {
                 p.out_scores[out + rank] = static_cast<float>(c.score);
-                p.out_tokens[out + rank] = c.place % p.V;
-                p.out_parents[out + rank] = c.place / p.V;
+                const int64_t w = c.place / p.V;
+                p.out_tokens[out + rank] = c.place - w * p.V;
+                p.out_parents[out + rank] = w;
             }
         }
         return;
     }
-    // More candidates above the edge than the list holds (many pieces whose best are all in a few of them): the best
-    // below the last one, n times.
+    // More candidates above the edge than the list holds (fewer lists than n, or many whose best are all in a few): the
+    // best below the last one, n times.
     Candidate last = {INFINITY, -1};
     for (int k = 0; k < p.n; ++k) {
         Candidate mine = {-INFINITY, -1};
-        for (int64_t i = tid; i < total; i += BJ_THREADS) {
-            const Candidate c = beam_candidate(p, b, i, s_base, s_kind);
-            if ((k == 0 || last.better(c)) && c.better(mine)) mine = c;
-        }
+        for (unsigned i = tid; i < lists; i += BJ_THREADS)
+            for (int e = 0; e < p.n; ++e) {
+                const Candidate c = beam_candidate(p, b, i / p.pieces, i % p.pieces, e, s_base, s_kind);
+                if (c.place < 0) break;
+                if (k > 0 && !last.better(c)) continue;            // taken already
+                if (c.better(mine)) mine = c;
+                break;
+            }
         __syncthreads();
         s_best[tid] = mine;
         __syncthreads();

@@ -24,6 +24,31 @@ __device__ __forceinline__ float warp_add(float v) {
     return v;
 }
 
+// Sum over a warp of a value per lane; every lane gets it.
+__device__ __forceinline__ int warp_add(int v) {
+#ifdef BT_SIMT_HOST
+    return warp_sum(v);
+#else
+    return __reduce_add_sync(0xffffffffu, v);
+#endif
+}
+// Threads that share a row of `units` pieces when a row is copied: a power of two, at most a warp.
+inline int row_lanes_log2(int units) {
+    int lg = 0;
+    while (lg < 5 && (1 << lg) < units) ++lg;
+    return lg;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {              // 2 ulp; -infinity gives 0
+#ifdef BT_SIMT_HOST
+    return exp2f(x);
+#else
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+#endif
+}
+
 // Launch that may start while its predecessor on the stream drains; the kernel calls pdl_wait() before it touches
 // global memory, so the call is stream-ordered like any other.
 template <typename Kern, typename Params>

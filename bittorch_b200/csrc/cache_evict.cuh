@@ -1,14 +1,17 @@
 // Eviction from a key/value cache by accumulated attention weight, and the gather of the slots that stay.
 //
 // evict_select: one CTA per sequence and key/value head finds the k-th largest weight among the slots that may go, as
-// a radix selection over the 32 ordered bits of a float (four passes of 8 bits, each a histogram in shared memory:
-// integer counts, so the order of the atomics does not matter), then writes the kept slots in order: a slot's place is
-// the number of kept slots before it, and of slots equal to the k-th weight the first ones stay.
+// a radix selection over the 32 ordered bits of a float (up to four passes of 8 bits), then writes the kept slots in
+// order: a slot's place is the number of kept slots before it, and of slots equal to the k-th weight the first ones
+// stay.  Weights have few exponents, so most slots of a warp count into the same digit: every lane has a column of the
+// histogram to itself, and no two lanes ever meet in a bank.  Counts are integers, so the order of the atomics does
+// not matter.  A thread holds neighbouring slots, in registers for the whole selection unless the cache is longer than
+// a CTA's registers.  Bound by latency (four passes of one CTA), not by the 4 bytes a slot.
 //
-// compact: rows are copied in units of 16 bytes (less where the alignment asks for it).  Between two caches every row
-// is independent.  In place, entry j goes to slot first + j <= keep[j], so a CTA takes a narrow column of one head's
-// cache (up to 64 bytes of every row) and walks the entries in blocks: all reads of a block, a barrier, then its
-// writes.  Reads of later blocks only touch slots that earlier writes do not reach.
+// compact: rows are copied in pieces of 16 bytes (less where the alignment asks for it), a row by neighbouring lanes.
+// Between two caches every row is independent.  In place, entry j goes to slot first + j <= keep[j], so a CTA takes a
+// narrow column of one head's cache (up to 64 bytes of every row) and walks the entries in blocks: all reads of a
+// block, a barrier, then its writes.  Reads of later blocks only touch slots that earlier writes do not reach.
 #pragma once
 
 #include "cache_common.cuh"
@@ -34,14 +37,17 @@ __device__ __forceinline__ uint32_t ordered_key(float x) {
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
+// IPT: neighbouring slots of a thread.
+template <int IPT>
 __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictParams p) {
-    __shared__ int s_hist[256];
-    __shared__ int s_scan[256];
+    constexpr int BLOCK = EV_THREADS * IPT;
+    __shared__ int s_hist[256 * 32];                               // [digit][lane]
+    __shared__ int s_digit[256];
     __shared__ unsigned s_warp[EV_THREADS / 32];
     __shared__ uint32_t s_prefix;
-    __shared__ int s_want;
+    __shared__ int s_want, s_left;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int h = static_cast<int>(blockIdx.x % p.Hkv), b = static_cast<int>(blockIdx.x / p.Hkv);
+    const int b = static_cast<int>(blockIdx.x / static_cast<unsigned>(p.Hkv)), h = static_cast<int>(blockIdx.x) - b * p.Hkv;
     pdl_launch_dependents();
     pdl_wait();
     const int n = p.lengths.at(b, p.S);
@@ -53,61 +59,107 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictPar
     }
     const float* mass = p.mass + b * p.mass_sb + h * p.mass_sh;
     const int lo = p.sinks, hi = n - p.recent;                     // the slots that compete
-    if (tid == 0) {
-        s_prefix = 0;
-        s_want = static_cast<int>(p.budget) - p.sinks - p.recent;
+    const int blocks = (n + BLOCK - 1) / BLOCK;
+    const bool vec = aligned(mass, 16);
+    uint32_t key[IPT];
+    auto load = [&](int i0) {
+        if (vec && i0 + IPT <= n) {
+#pragma unroll
+            for (int i = 0; i < IPT; i += 4) {
+                const float4 x = *reinterpret_cast<const float4*>(mass + i0 + i);
+                key[i] = ordered_key(x.x); key[i + 1] = ordered_key(x.y); key[i + 2] = ordered_key(x.z); key[i + 3] = ordered_key(x.w);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < IPT; ++i) key[i] = i0 + i < n ? ordered_key(mass[i0 + i]) : 0;
+        }
+    };
+    if (blocks == 1) load(tid * IPT);
+    uint32_t prefix = 0;                                           // the digits of the k-th largest key that are known
+    int want = static_cast<int>(p.budget) - p.sinks - p.recent;    // it is the want-th largest of those with this prefix
+    int shift = 32;                                                // bits not yet known
+    while (want > 0 && shift > 0) {
+        shift -= 8;
+        for (int i = tid; i < 256 * 32; i += EV_THREADS) s_hist[i] = 0;
+        __syncthreads();
+        for (int blk = 0; blk < blocks; ++blk) {
+            const int i0 = blk * BLOCK + tid * IPT;
+            if (blocks > 1) load(i0);
+#pragma unroll
+            for (int i = 0; i < IPT; ++i)
+                if (i0 + i >= lo && i0 + i < hi && (shift == 24 || ((key[i] ^ prefix) >> (shift + 8)) == 0))
+                    atomicAdd(&s_hist[((key[i] >> shift) & 255u) * 32 + lane], 1);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 256 / (EV_THREADS / 32); ++i) {
+            const int d = warp * (256 / (EV_THREADS / 32)) + i, sum = warp_add(s_hist[d * 32 + lane]);
+            if (lane == 0) s_digit[d] = sum;
+        }
+        __syncthreads();
+        if (warp == 0) {                                           // eight digits per lane, the largest in lane 31
+            int mine = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) mine += s_digit[lane * 8 + i];
+            int above = mine;                                      // inclusive, from the top
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_down_sync(0xffffffffu, above, o);
+                if (lane + o < 32) above += x;
+            }
+            above -= mine;
+            if (above < want && above + mine >= want) {            // one lane
+                int d = lane * 8 + 7;
+                while (above + s_digit[d] < want) above += s_digit[d--];
+                s_prefix = prefix | (static_cast<uint32_t>(d) << shift);
+                s_want = want - above;
+                s_left = s_digit[d];
+            }
+        }
+        __syncthreads();
+        prefix = s_prefix;
+        want = s_want;
+        if (s_left == want) break;                                 // all of them stay: the lower bits do not matter
     }
-    __syncthreads();
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (s_want == 0) break;                                    // nothing of the middle stays
-        if (tid < 256) s_hist[tid] = 0;
-        __syncthreads();
-        const uint32_t prefix = s_prefix;
-        for (int i = lo + tid; i < hi; i += EV_THREADS) {
-            const uint32_t key = ordered_key(mass[i]);
-            if (shift == 24 || ((key ^ prefix) >> (shift + 8)) == 0) atomicAdd(&s_hist[(key >> shift) & 255u], 1);
+    const int equal_kept = want;                                   // so many of those that tie with the prefix stay, the first ones
+    const bool none = static_cast<int>(p.budget) == p.sinks + p.recent;
+    int above = 0, equal = 0;                                      // kept / tying slots before this block
+    for (int blk = 0; blk < blocks; ++blk) {
+        const int i0 = blk * BLOCK + tid * IPT;
+        if (blocks > 1) load(i0);
+        unsigned stays = 0, ties = 0;                              // a bit per slot
+#pragma unroll
+        for (int i = 0; i < IPT; ++i) {
+            const int s = i0 + i;
+            const bool middle = s >= lo && s < hi && !none;
+            if ((s < n && (s < lo || s >= hi)) || (middle && (key[i] >> shift) > (prefix >> shift))) stays |= 1u << i;
+            if (middle && (key[i] >> shift) == (prefix >> shift)) ties |= 1u << i;
         }
-        __syncthreads();
-        // s_scan[i]: how many keys of this prefix have a digit >= i
-        if (tid < 256) s_scan[tid] = s_hist[tid];
-        for (int step = 1; step < 256; step <<= 1) {
-            __syncthreads();
-            const int add = tid + step < 256 ? s_scan[tid + step] : 0;
-            __syncthreads();
-            if (tid < 256) s_scan[tid] += add;
+        const unsigned mine = static_cast<unsigned>(__popc(stays)) | (static_cast<unsigned>(__popc(ties)) << 16);     // a block holds at most 2^14 of each
+        unsigned upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
         }
+        if (lane == 31) s_warp[warp] = upto;
         __syncthreads();
-        const int want = s_want;
-        __syncthreads();
-        if (tid < 256 && s_scan[tid] >= want && s_scan[tid] - s_hist[tid] < want) {     // one digit holds the k-th key
-            s_prefix = prefix | (static_cast<uint32_t>(tid) << shift);
-            s_want = want - (s_scan[tid] - s_hist[tid]);
+        unsigned all = s_warp[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned x = __shfl_up_sync(0xffffffffu, all, o);
+            if (lane >= o) all += x;
         }
-        __syncthreads();
-    }
-    const uint32_t edge = s_prefix;                                // the k-th largest key; s_want slots equal to it stay
-    const int equal_kept = s_want;
-    const bool none = p.budget - p.sinks - p.recent == 0;
-    int above = 0, equal = 0;                                      // kept / equal-to-the-edge slots before this block of slots
-    for (int i0 = 0; i0 < n; i0 += EV_THREADS) {
-        const int i = i0 + tid;
-        bool stays = i < n && (i < lo || i >= hi), ties = false;
-        if (i >= lo && i < hi && !none) {
-            const uint32_t key = ordered_key(mass[i]);
-            stays = key > edge;
-            ties = key == edge;
+        const unsigned before = (warp > 0 ? __shfl_sync(0xffffffffu, all, warp > 0 ? warp - 1 : 0) : 0u) + upto - mine;
+        const unsigned total = __shfl_sync(0xffffffffu, all, 31);
+        int a = above + static_cast<int>(before & 0xffffu), e = equal + static_cast<int>(before >> 16);
+#pragma unroll
+        for (int i = 0; i < IPT; ++i) {
+            const bool st = (stays >> i) & 1u, tie = (ties >> i) & 1u;
+            if (st || (tie && e < equal_kept)) keep[a + (e < equal_kept ? e : equal_kept)] = i0 + i;
+            a += st;
+            e += tie;
         }
-        const unsigned ms = __ballot_sync(0xffffffffu, stays), mt = __ballot_sync(0xffffffffu, ties), below = (1u << lane) - 1;
-        if (lane == 0) s_warp[warp] = static_cast<unsigned>(__popc(ms)) | (static_cast<unsigned>(__popc(mt)) << 16);
-        __syncthreads();
-        unsigned before = 0, total = 0;                            // both counts stay below 2^16: a block is 1024 slots
-        for (int w = 0; w < EV_THREADS / 32; ++w) {
-            if (w == warp) before = total;
-            total += s_warp[w];
-        }
-        const int a = above + static_cast<int>(before & 0xffffu) + __popc(ms & below);
-        const int e = equal + static_cast<int>(before >> 16) + __popc(mt & below);
-        if (stays || (ties && e < equal_kept)) keep[a + min(e, equal_kept)] = i;
         above += static_cast<int>(total & 0xffffu);
         equal += static_cast<int>(total >> 16);
         __syncthreads();
@@ -125,7 +177,7 @@ struct CompactParams {
     const float* mass;
     float* mass_out;
     int64_t msb, msh, mdb, mdh;                                    // in elements
-    int B, Hkv, S, S_out, units;                                   // units of a row
+    int B, Hkv, S, S_out, units, lanes_log2;                       // units of a row, threads of a row
     int64_t n;
     int blocks;                                                    // gather: CTAs per sequence, head and tensor
 };
@@ -136,20 +188,18 @@ __device__ __forceinline__ int64_t compact_count(const CompactParams& p, int b) 
 }
 
 constexpr int CG_THREADS = 256;
-constexpr int CG_UNITS = 4;                                        // copies in flight per thread
+constexpr int CG_ROWS = 4;                                         // rows in flight per thread
 
 // Between two caches: blockIdx.y = tensor (0, 1) or the mass (2).
 template <typename U>
 __global__ void __launch_bounds__(CG_THREADS) compact_gather_kernel(const CompactParams p) {
     const int tid = threadIdx.x;
-    const int64_t bh = blockIdx.x / p.blocks;
-    const int blk = static_cast<int>(blockIdx.x % p.blocks);
-    const int h = static_cast<int>(bh % p.Hkv), b = static_cast<int>(bh / p.Hkv);
+    const int bh = static_cast<int>(blockIdx.x / static_cast<unsigned>(p.blocks)), blk = static_cast<int>(blockIdx.x) - bh * p.blocks;
+    const int b = bh / p.Hkv, h = bh - b * p.Hkv, which = blockIdx.y;
     pdl_launch_dependents();
     pdl_wait();
     const int64_t count = compact_count(p, b), first = p.first ? p.first[b] : 0;
     const int64_t* keep = p.keep + b * p.keep_sb + h * p.keep_sh;
-    const int which = blockIdx.y;
     if (which == 2) {
         const float* m = p.mass + b * p.msb + h * p.msh;
         float* out = p.mass_out + b * p.mdb + h * p.mdh;
@@ -163,23 +213,25 @@ __global__ void __launch_bounds__(CG_THREADS) compact_gather_kernel(const Compac
     }
     const uint8_t* src = p.src[which] + b * p.sb[which] + h * p.sh[which];
     uint8_t* dst = p.dst[which] + b * p.db[which] + h * p.dh[which];
-    const int64_t total = count * p.units, step = static_cast<int64_t>(p.blocks) * CG_THREADS;
-    for (int64_t u0 = blk * static_cast<int64_t>(CG_THREADS) + tid; u0 < total; u0 += step * CG_UNITS) {
-        U v[CG_UNITS];
-        U* to[CG_UNITS];
+    const int64_t ss = p.ss[which], ds = p.ds[which];
+    const int rows = CG_THREADS >> p.lanes_log2, c0 = tid & ((1 << p.lanes_log2) - 1);
+    for (int64_t j0 = static_cast<int64_t>(blk) * rows * CG_ROWS + (tid >> p.lanes_log2); j0 < count; j0 += static_cast<int64_t>(p.blocks) * rows * CG_ROWS) {
+        int64_t from[CG_ROWS];
 #pragma unroll
-        for (int i = 0; i < CG_UNITS; ++i) {
-            const int64_t u = u0 + i * step;
-            to[i] = nullptr;
-            if (u >= total) continue;
-            const int64_t j = u / p.units, c = u - j * p.units, from = keep[j], at = first + j;
-            if (from < 0 || from >= p.S || at < 0 || at >= p.S_out) continue;
-            v[i] = *reinterpret_cast<const U*>(src + from * p.ss[which] + c * sizeof(U));
-            to[i] = reinterpret_cast<U*>(dst + at * p.ds[which] + c * sizeof(U));
+        for (int i = 0; i < CG_ROWS; ++i) {
+            const int64_t j = j0 + i * rows, at = first + j;
+            from[i] = j < count && at >= 0 && at < p.S_out ? keep[j] : -1;
+            if (from[i] >= p.S) from[i] = -1;
         }
+        for (int c = c0; c < p.units; c += 1 << p.lanes_log2) {
+            U v[CG_ROWS];
 #pragma unroll
-        for (int i = 0; i < CG_UNITS; ++i)
-            if (to[i] != nullptr) *to[i] = v[i];
+            for (int i = 0; i < CG_ROWS; ++i)
+                if (from[i] >= 0) v[i] = *reinterpret_cast<const U*>(src + from[i] * ss + c * sizeof(U));
+#pragma unroll
+            for (int i = 0; i < CG_ROWS; ++i)
+                if (from[i] >= 0) *reinterpret_cast<U*>(dst + (first + j0 + i * rows) * ds + c * sizeof(U)) = v[i];
+        }
     }
 }
 
@@ -244,9 +296,10 @@ static int launch_compact(CompactParams p, bool in_place, int row_bytes, void* s
     if (in_place)
         return launch_early(compact_inplace_kernel<U>, "compact_inplace_kernel",
                             dim3(static_cast<unsigned>(heads * ceil_div(p.units, CI_COLS)), kinds), CI_THREADS, 0, stream, p);
-    // as many CTAs as keep every SM at eight, each with at least one full round of copies
-    int64_t blocks = ceil_div<int64_t>(p.n * p.units, CG_THREADS * CG_UNITS);
-    blocks = std::min<int64_t>(blocks, std::max<int64_t>(1, ceil_div<int64_t>(static_cast<int64_t>(sm_count()) * 8, heads * 2)));
+    // up to four waves of eight CTAs per SM, each with at least one full round of copies
+    p.lanes_log2 = row_lanes_log2(p.units);
+    int64_t blocks = ceil_div<int64_t>(p.n, (CG_THREADS >> p.lanes_log2) * CG_ROWS);
+    blocks = std::min<int64_t>(blocks, std::max<int64_t>(1, ceil_div<int64_t>(static_cast<int64_t>(sm_count()) * 32, heads * 2)));
     p.blocks = static_cast<int>(std::max<int64_t>(1, blocks));
     return launch_early(compact_gather_kernel<U>, "compact_gather_kernel", dim3(static_cast<unsigned>(heads * p.blocks), kinds), CG_THREADS, 0, stream, p);
 }
@@ -270,7 +323,9 @@ extern "C" int bt_evict_select(const float* mass, int64_t mass_sb, int64_t mass_
     p.S = static_cast<int>(S); p.Hkv = static_cast<int>(Hkv);
     p.sinks = static_cast<int>(sinks); p.recent = static_cast<int>(recent);
     p.budget = budget; p.keep = keep; p.counts = counts;
-    return launch_early(evict_select_kernel, "evict_select_kernel", dim3(static_cast<unsigned>(B * Hkv)), EV_THREADS, 0, stream, p);
+    const dim3 grid(static_cast<unsigned>(B * Hkv));
+    if (S <= 4 * EV_THREADS) return launch_early(evict_select_kernel<4>, "evict_select_kernel", grid, EV_THREADS, 0, stream, p);
+    return launch_early(evict_select_kernel<16>, "evict_select_kernel", grid, EV_THREADS, 0, stream, p);
 }
 
 extern "C" int bt_compact_cache(const void* k, const void* v, void* k_out, void* v_out, int dtype, int64_t B, int64_t Hkv,

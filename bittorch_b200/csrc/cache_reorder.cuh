@@ -19,7 +19,7 @@ struct ReorderParams {
     int64_t row[RO_TENSORS], head[RO_TENSORS], slot[RO_TENSORS];   // strides in bytes
     const int64_t* parents;
     Lengths lengths;
-    int W, Hkv, S, start, units;
+    int W, Hkv, S, start, units, lanes_log2;
     int blocks;                                                    // CTAs per tensor, group and head
 };
 
@@ -27,8 +27,8 @@ template <typename U, int WMAX>
 __global__ void __launch_bounds__(RO_THREADS) reorder_cache_kernel(const __grid_constant__ ReorderParams p) {
     __shared__ int s_parent[WMAX];
     const int tid = threadIdx.x;
-    const int64_t at = blockIdx.x / p.blocks;
-    const int blk = static_cast<int>(blockIdx.x % p.blocks), h = static_cast<int>(at % p.Hkv), b = static_cast<int>(at / p.Hkv), t = blockIdx.y;
+    const int at = static_cast<int>(blockIdx.x / static_cast<unsigned>(p.blocks)), blk = static_cast<int>(blockIdx.x) - at * p.blocks;
+    const int b = at / p.Hkv, h = at - b * p.Hkv, t = blockIdx.y;
     pdl_launch_dependents();
     pdl_wait();
     if (tid < WMAX) {
@@ -41,18 +41,19 @@ __global__ void __launch_bounds__(RO_THREADS) reorder_cache_kernel(const __grid_
     for (int w = 0; w < WMAX; ++w) parent[w] = s_parent[w];
     const int end = p.lengths.at(b, p.S);
     uint8_t* base = p.base[t] + static_cast<int64_t>(b) * p.W * p.row[t] + h * p.head[t];
-    const int64_t total = end > p.start ? static_cast<int64_t>(end - p.start) * p.units : 0;
-    for (int64_t u = blk * static_cast<int64_t>(RO_THREADS) + tid; u < total; u += static_cast<int64_t>(p.blocks) * RO_THREADS) {
-        const int64_t n = u / p.units, c = u - n * p.units;
-        uint8_t* place = base + (p.start + n) * p.slot[t] + c * sizeof(U);
-        U v[WMAX];
+    const int64_t row = p.row[t], slot = p.slot[t];
+    const int lanes = 1 << p.lanes_log2, rows = RO_THREADS >> p.lanes_log2;
+    for (int64_t n = p.start + static_cast<int64_t>(blk) * rows + (tid >> p.lanes_log2); n < end; n += static_cast<int64_t>(p.blocks) * rows)
+        for (int c = tid & (lanes - 1); c < p.units; c += lanes) {
+            uint8_t* place = base + n * slot + c * sizeof(U);
+            U v[WMAX];
 #pragma unroll
-        for (int w = 0; w < WMAX; ++w)
-            if (parent[w] != w) v[w] = *reinterpret_cast<const U*>(place + parent[w] * p.row[t]);
+            for (int w = 0; w < WMAX; ++w)
+                if (parent[w] != w) v[w] = *reinterpret_cast<const U*>(place + parent[w] * row);
 #pragma unroll
-        for (int w = 0; w < WMAX; ++w)
-            if (parent[w] != w) *reinterpret_cast<U*>(place + w * p.row[t]) = v[w];
-    }
+            for (int w = 0; w < WMAX; ++w)
+                if (parent[w] != w) *reinterpret_cast<U*>(place + w * row) = v[w];
+        }
 }
 
 template <typename U>
@@ -61,7 +62,8 @@ static int launch_reorder(ReorderParams p, int64_t tensors, int64_t B, int row_b
     const int64_t heads = B * p.Hkv;
     // enough CTAs for 16 rounds of every SM over the whole launch, no more than there are places
     int64_t blocks = ceil_div<int64_t>(static_cast<int64_t>(sm_count()) * 8 * 16, heads * tensors);
-    blocks = std::min<int64_t>(blocks, ceil_div<int64_t>(static_cast<int64_t>(p.S - p.start) * p.units, RO_THREADS));
+    p.lanes_log2 = row_lanes_log2(p.units);
+    blocks = std::min<int64_t>(blocks, ceil_div<int64_t>(p.S - p.start, RO_THREADS >> p.lanes_log2));
     p.blocks = static_cast<int>(std::max<int64_t>(1, blocks));
     const dim3 grid(static_cast<unsigned>(heads * p.blocks), static_cast<unsigned>(tensors));
     if (p.W <= 4) return launch_early(reorder_cache_kernel<U, 4>, "reorder_cache_kernel", grid, RO_THREADS, 0, stream, p);

@@ -21,13 +21,19 @@ from torch import Tensor
 from .._ext import require_ext
 
 
+_bound = None
+
+
 def _binding():
-    require_ext()
-    try:
-        from .. import _cache
-    except ImportError as exc:
-        raise RuntimeError(f"bittorch_b200: {exc}") from exc
-    return _cache
+    global _bound
+    if _bound is None:
+        require_ext()
+        try:
+            from .. import _cache
+        except ImportError as exc:
+            raise RuntimeError(f"bittorch_b200: {exc}") from exc
+        _bound = _cache
+    return _bound
 
 
 def tree_mask(parents: Tensor) -> Tensor:

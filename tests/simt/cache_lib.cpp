@@ -23,8 +23,14 @@ inline unsigned __ballot_sync(unsigned, bool on) {
     pthread_barrier_wait(&w.bar);
     return r;
 }
+template <typename T> inline T __shfl_sync(unsigned, T v, int src) { return ::simt::shfl(v, src); }
+template <typename T> inline T __shfl_up_sync(unsigned, T v, int by) { return ::simt::shfl(v, ::simt::my_lane() >= by ? ::simt::my_lane() - by : ::simt::my_lane()); }
+template <typename T> inline T __shfl_down_sync(unsigned, T v, int by) { return ::simt::shfl(v, ::simt::my_lane() + by < 32 ? ::simt::my_lane() + by : ::simt::my_lane()); }
 #ifndef __grid_constant__
 #define __grid_constant__
+#endif
+#ifndef __noinline__
+#define __noinline__ __attribute__((noinline))
 #endif
 
 #include <cstdarg>
