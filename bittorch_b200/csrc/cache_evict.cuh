@@ -74,21 +74,31 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictPar
             for (int i = 0; i < IPT; ++i) key[i] = i0 + i < n ? ordered_key(mass[i0 + i]) : 0;
         }
     };
-    if (blocks == 1) load(tid * IPT);
+    // Slots that do not compete count as the lowest key there is: they never stand above another, and where the k-th key
+    // is that low (a NaN's), the last loop leaves them out.
+    auto competitors = [&](int i0) {
+        load(i0);
+        if (i0 < lo || i0 + IPT > hi) {
+#pragma unroll
+            for (int i = 0; i < IPT; ++i)
+                if (i0 + i < lo || i0 + i >= hi) key[i] = 0;
+        }
+    };
+    if (blocks == 1) competitors(tid * IPT);
     uint32_t prefix = 0;                                           // the digits of the k-th largest key that are known
     int want = static_cast<int>(p.budget) - p.sinks - p.recent;    // it is the want-th largest of those with this prefix
     int shift = 32;                                                // bits not yet known
-    while (want > 0 && shift > 0) {
-        shift -= 8;
+#pragma unroll
+    for (int pass = 0; pass < 4; ++pass) {
+        if (want == 0) break;
+        shift = 24 - 8 * pass;
         for (int i = tid; i < 256 * 32; i += EV_THREADS) s_hist[i] = 0;
         __syncthreads();
         for (int blk = 0; blk < blocks; ++blk) {
-            const int i0 = blk * BLOCK + tid * IPT;
-            if (blocks > 1) load(i0);
+            if (blocks > 1) competitors(blk * BLOCK + tid * IPT);
 #pragma unroll
             for (int i = 0; i < IPT; ++i)
-                if (i0 + i >= lo && i0 + i < hi && (shift == 24 || ((key[i] ^ prefix) >> (shift + 8)) == 0))
-                    atomicAdd(&s_hist[((key[i] >> shift) & 255u) * 32 + lane], 1);
+                if (pass == 0 || (key[i] >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&s_hist[((key[i] >> shift) & 255u) * 32 + lane], 1);
         }
         __syncthreads();
 #pragma unroll
@@ -123,19 +133,24 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictPar
     }
     const int equal_kept = want;                                   // so many of those that tie with the prefix stay, the first ones
     const bool none = static_cast<int>(p.budget) == p.sinks + p.recent;
+    const uint32_t edge = shift < 32 ? prefix >> shift : 0;
+    shift &= 31;                                                   // nothing competes where it is 32
     int above = 0, equal = 0;                                      // kept / tying slots before this block
     for (int blk = 0; blk < blocks; ++blk) {
         const int i0 = blk * BLOCK + tid * IPT;
-        if (blocks > 1) load(i0);
+        if (blocks > 1) competitors(i0);
         unsigned stays = 0, ties = 0;                              // a bit per slot
 #pragma unroll
         for (int i = 0; i < IPT; ++i) {
-            const int s = i0 + i;
-            const bool middle = s >= lo && s < hi && !none;
-            if ((s < n && (s < lo || s >= hi)) || (middle && (key[i] >> shift) > (prefix >> shift))) stays |= 1u << i;
-            if (middle && (key[i] >> shift) == (prefix >> shift)) ties |= 1u << i;
+            if ((key[i] >> shift) > edge) stays |= 1u << i;
+            if ((key[i] >> shift) == edge) ties |= 1u << i;
         }
-        const unsigned mine = static_cast<unsigned>(__popc(stays)) | (static_cast<unsigned>(__popc(ties)) << 16);     // a block holds at most 2^14 of each
+        // bits of the slots below x among this thread's
+        auto below = [&](int x) { return x <= i0 ? 0u : x >= i0 + IPT ? ~0u : (1u << (x - i0)) - 1u; };
+        const unsigned compete = below(hi) & ~below(lo), exist = below(n) & (IPT == 32 ? ~0u : (1u << (IPT & 31)) - 1u);
+        stays = none ? exist & ~compete : ((stays & compete) | ~compete) & exist;
+        ties = none ? 0u : ties & compete & exist;
+        const unsigned mine = static_cast<unsigned>(__popc(stays)) | (static_cast<unsigned>(__popc(ties)) << 16);     // a block holds at most 2^15 of each
         unsigned upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -153,11 +168,11 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictPar
         const unsigned before = (warp > 0 ? __shfl_sync(0xffffffffu, all, warp > 0 ? warp - 1 : 0) : 0u) + upto - mine;
         const unsigned total = __shfl_sync(0xffffffffu, all, 31);
         int a = above + static_cast<int>(before & 0xffffu), e = equal + static_cast<int>(before >> 16);
-#pragma unroll
-        for (int i = 0; i < IPT; ++i) {
-            const bool st = (stays >> i) & 1u, tie = (ties >> i) & 1u;
-            if (st || (tie && e < equal_kept)) keep[a + (e < equal_kept ? e : equal_kept)] = i0 + i;
-            a += st;
+        for (unsigned left = stays | ties; left != 0; left &= left - 1) {
+            const int i = __ffs(left) - 1;
+            const bool tie = (ties >> i) & 1u;
+            if (!tie || e < equal_kept) keep[a + (e < equal_kept ? e : equal_kept)] = i0 + i;
+            a += !tie;
             e += tie;
         }
         above += static_cast<int>(total & 0xffffu);
@@ -324,8 +339,10 @@ extern "C" int bt_evict_select(const float* mass, int64_t mass_sb, int64_t mass_
     p.sinks = static_cast<int>(sinks); p.recent = static_cast<int>(recent);
     p.budget = budget; p.keep = keep; p.counts = counts;
     const dim3 grid(static_cast<unsigned>(B * Hkv));
+    // the shortest run of slots per thread that holds the cache in registers; a longer cache is read again in every pass
     if (S <= 4 * EV_THREADS) return launch_early(evict_select_kernel<4>, "evict_select_kernel", grid, EV_THREADS, 0, stream, p);
-    return launch_early(evict_select_kernel<16>, "evict_select_kernel", grid, EV_THREADS, 0, stream, p);
+    if (S <= 16 * EV_THREADS) return launch_early(evict_select_kernel<16>, "evict_select_kernel", grid, EV_THREADS, 0, stream, p);
+    return launch_early(evict_select_kernel<32>, "evict_select_kernel", grid, EV_THREADS, 0, stream, p);
 }
 
 extern "C" int bt_compact_cache(const void* k, const void* v, void* k_out, void* v_out, int dtype, int64_t B, int64_t Hkv,

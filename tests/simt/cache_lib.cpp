@@ -13,6 +13,7 @@ inline int atomicAdd(int* p, int v) {
     *p = old + v;
     return old;
 }
+inline int __ffs(int v) { return __builtin_ffs(v); }
 inline int __popc(unsigned v) { return __builtin_popcount(v); }
 inline unsigned __ballot_sync(unsigned, bool on) {
     simt::Warp& w = simt::my_warp();
