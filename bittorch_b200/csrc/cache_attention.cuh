@@ -332,12 +332,24 @@ __global__ void __launch_bounds__(AM_THREADS) attn_merge_kernel(const AttnParams
 // How a call is cut up; the workspace size follows from it.
 struct AttnPlan {
     int row_tiles, nsplit;
-    size_t o_bytes, ml_bytes, score_bytes;
-    size_t bytes() const { return o_bytes + ml_bytes + score_bytes; }
+    size_t o_bytes, ml_bytes, score_bytes, tc_bytes;
+    size_t bytes() const { return std::max(o_bytes + ml_bytes + score_bytes, tc_bytes); }
 };
 
-static AttnPlan attn_plan(int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t S, int64_t D, bool want_mass) {
+// cache_attention_tcgen05.cuh
+static bool attn_tc_sizes(int64_t H, int64_t Hkv, int64_t T, int64_t D, int dtype, bool want_mass);
+static size_t attn_tc_bytes(int64_t D);
+static bool attn_tc_ok(const AttnParams& p);
+static int launch_attn_tc_for(const AttnParams& a, int dtype, float scale, void* workspace, void* stream);
+
+static AttnPlan attn_plan(int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t S, int64_t D, int dtype, bool want_mass) {
     AttnPlan a;
+#ifdef BT_SIMT_HOST
+    a.tc_bytes = 0;
+    (void)dtype;
+#else
+    a.tc_bytes = attn_tc_sizes(H, Hkv, T, D, dtype, want_mass) ? attn_tc_bytes(D) : 0;
+#endif
     const int64_t rows = H / Hkv * T;
     a.row_tiles = static_cast<int>(ceil_div<int64_t>(rows, AT_ROWS));
     const int64_t units = B * Hkv * a.row_tiles;
@@ -397,7 +409,7 @@ extern "C" size_t bt_tree_attention_workspace(int64_t B, int64_t H, int64_t Hkv,
                                               int want_mass) {
     using namespace bt;
     if (!attn_sizes_ok(B, H, Hkv, T, S, D) || !attn_sizes_supported(B, H, Hkv, T, S, D) || !valid_dtype(dtype)) return 0;
-    return attn_plan(B, H, Hkv, T, S, D, want_mass != 0).bytes();
+    return attn_plan(B, H, Hkv, T, S, D, dtype, want_mass != 0).bytes();
 }
 
 extern "C" int bt_tree_attention(const void* q, const void* k, const void* v, int dtype, int64_t B, int64_t H, int64_t Hkv,
@@ -413,7 +425,7 @@ extern "C" int bt_tree_attention(const void* q, const void* k, const void* v, in
     BT_REQUIRE(scale == scale && scale - scale == 0.0f, "bt_tree_attention: scale must be finite");
     BT_UNSUPPORTED_IF(!attn_sizes_supported(B, H, Hkv, T, S, D), "bt_tree_attention: sizes too large (head size at most %d)",
                       BT_ATTENTION_MAX_D);
-    const AttnPlan plan = attn_plan(B, H, Hkv, T, S, D, mass != nullptr);
+    const AttnPlan plan = attn_plan(B, H, Hkv, T, S, D, dtype, mass != nullptr);
     BT_REQUIRE(workspace_bytes >= plan.bytes(), "bt_tree_attention: workspace of %zu bytes, %zu needed", workspace_bytes, plan.bytes());
     BT_REQUIRE(plan.bytes() == 0 || (workspace != nullptr && aligned(workspace, 16)), "bt_tree_attention: workspace must be 16-byte aligned");
     AttnParams p = {};
@@ -437,6 +449,9 @@ extern "C" int bt_tree_attention(const void* q, const void* k, const void* v, in
     const size_t four = 4 * dtype_size(dtype);
     p.vec = D % 4 == 0 && aligned(q, four) && aligned(k, four) && aligned(v, four);
     for (int i = 0; i < 9; ++i) p.vec = p.vec && strides[i] % 4 == 0;
+#ifndef BT_SIMT_HOST
+    if (plan.tc_bytes != 0 && attn_tc_ok(p)) return launch_attn_tc_for(p, dtype, scale, workspace, stream);
+#endif
     if (dtype == BT_F32) return launch_attention<float>(p, plan, stream);
     if (dtype == BT_F16) return launch_attention<__half>(p, plan, stream);
     return launch_attention<__nv_bfloat16>(p, plan, stream);

@@ -1,0 +1,639 @@
+// The 16-bit kernel of bt_tree_attention for many rows per key/value head (token trees, grouped heads): both products on the
+// 5th-generation tensor cores, scores, weights and output in tensor memory.
+//
+// The rows of a head (query heads x new tokens) are cut into tiles of 128, one thread per row.  A CTA works on two tiles
+// of one sequence at a time ("streams"): while the tensor cores make one tile's scores, the other tile's threads turn
+// theirs into weights.  Tiles of the same head share the keys and values that TMA brings in; the last tile of a head and
+// the first of the next go together too, each with its own.  A stream's step, for 128 slots:
+//   S = Q K^T   tcgen05.mma, both operands in shared memory, 128 columns of TMEM
+//   weights     a row's 128 scores in its thread's registers; the reference point of the exponentials moves only when a
+//               score exceeds it by 2^8 (the sums stay far from overflow, and the output is almost never rescaled);
+//               the weights, rounded to the cache's type, go back into TMEM where the scores were
+//   O += P V    tcgen05.mma with P from TMEM, V as it lies in the cache (its columns contiguous)
+//
+// Work is dealt out in blocks of 128 slots: the blocks of all pairs of tiles of all sequences form one line, and every
+// CTA (one per SM) takes an equal piece of it, so that ragged lengths cost nothing.  A CTA writes a pair that it has
+// whole straight to the output; of the others, the first and the last of its piece, it leaves sums, maxima and
+// unnormalised output in its two places of the workspace, and attn_tc_join_kernel adds the pieces of a pair up.
+//
+// New tokens: scores that a row does not see are masked; values in slots past the end are overwritten with zeros before
+// they are multiplied, and so are infinities and NaN among the new tokens' values, which are added at the end to
+// the rows that see them.  Bound by the tensor cores from about 128 rows on, by HBM below.
+#pragma once
+
+#include "cache_attention_stream.cuh"
+#include "gemm_tcgen05.cuh"
+
+namespace bt {
+
+constexpr int TC_ROWS = 128;                                       // rows of a tile
+constexpr int TC_KEYS = 128;                                       // slots of a block
+constexpr int TC_SLOTS = 4;                                        // ring of key / value tiles
+constexpr int TC_THREADS = 384;                                    // warps: 0 TMA, 1 MMA, 2-3 values of new tokens, 4-7 and 8-11 the streams
+constexpr int TC_COLS = 512;                                       // TMEM: S0 at 0, S1 at 128, O0 at 256, O1 at 384
+constexpr float TC_LAZY = 8.0f;                                    // how far (in powers of 2) a score may exceed the reference point
+
+template <int D> __host__ __device__ constexpr int tc_tile_bytes() { return TC_KEYS * D * 2; }
+template <int D> constexpr size_t tc_smem() { return 1024 + static_cast<size_t>(2 + TC_SLOTS) * tc_tile_bytes<D>() + 1024; }
+
+struct AttnTcParams {
+    AttnParams a;
+    int tiles;                                                     // of a head
+    int items;                                                     // Hkv * tiles of a sequence
+    int pairs;                                                     // pairs of tiles of a sequence
+    float scale2;                                                  // |scale| * log2(e)
+    int flip;                                                      // scale < 0: queries are negated instead
+    float* part_o;                                                 // [CTA][2][stream][128][D]
+    float2* part_ml;                                               // [CTA][2][stream][128]
+};
+
+// A piece of one pair's line of blocks
+struct TcPiece {
+    int b, pair, k0, k1, blocks, len, end;
+    __device__ __forceinline__ bool whole() const { return k0 == 0 && k1 == blocks; }
+};
+__device__ __forceinline__ int tc_blocks(const AttnTcParams& p, int b) { return (attn_end(p.a, attn_len(p.a, b)) + TC_KEYS - 1) / TC_KEYS; }
+
+// Blocks of the whole line, and where position `pos` lies on it.  Run by whole warps; every lane gets the result.
+__device__ __forceinline__ int64_t tc_total(const AttnTcParams& p) {
+    const int lane = threadIdx.x & 31;
+    int64_t sum = 0;
+    for (int b = lane; b < p.a.B; b += 32) sum += tc_blocks(p, b);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum * p.pairs;
+}
+__device__ __forceinline__ void tc_locate(const AttnTcParams& p, int64_t pos, int& b, int& pair, int& block) {
+    const int lane = threadIdx.x & 31;
+    int64_t before = 0;
+    b = p.a.B, pair = 0, block = 0;
+    for (int b0 = 0; b0 < p.a.B; b0 += 32) {
+        const int n = b0 + lane < p.a.B ? tc_blocks(p, b0 + lane) : 0;
+        int64_t upto = static_cast<int64_t>(n) * p.pairs;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, before + upto > pos);
+        if (past != 0) {
+            const int hit = __ffs(past) - 1;
+            const int blocks = __shfl_sync(0xffffffffu, n, hit);
+            const int64_t start = before + __shfl_sync(0xffffffffu, upto, hit) - static_cast<int64_t>(blocks) * p.pairs;
+            b = b0 + hit;
+            pair = static_cast<int>((pos - start) / blocks);
+            block = static_cast<int>((pos - start) - static_cast<int64_t>(pair) * blocks);
+            return;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+}
+// Where CTA i's piece of the line begins
+struct TcCuts {
+    int64_t each;
+    unsigned rest, ctas;
+    __device__ __forceinline__ TcCuts(int64_t total, unsigned n) : each(total / n), rest(static_cast<unsigned>(total % n)), ctas(n) {}
+    __device__ __forceinline__ int64_t at(unsigned i) const { return each * i + rest * i / ctas; }
+};
+
+struct TcWalk {
+    int b, pair, block;
+    int64_t left;
+    __device__ __forceinline__ bool next(const AttnTcParams& p, TcPiece& c) {
+        if (left <= 0 || b >= p.a.B) return false;
+        c.b = b; c.pair = pair; c.k0 = block;
+        c.len = attn_len(p.a, b);
+        c.end = attn_end(p.a, c.len);
+        c.blocks = (c.end + TC_KEYS - 1) / TC_KEYS;
+        c.k1 = static_cast<int>(c.blocks - block < left ? c.blocks : block + left);
+        left -= c.k1 - c.k0;
+        block = 0;
+        if (++pair == p.pairs) pair = 0, ++b;
+        return true;
+    }
+};
+
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+        ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+        : "memory");
+}
+__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+                   "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Operand whose columns (not the summed dimension) are contiguous, 128-byte swizzle: 64 columns x 8 rows per 1024 bytes,
+// row groups 1024 bytes apart, groups of 64 columns a tile of 128 rows apart
+__device__ __forceinline__ uint64_t umma_desc_sw128_mn(uint32_t smem_addr) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((smem_addr & 0x3ffffu) >> 4);
+    d |= static_cast<uint64_t>((TC_KEYS * 128) >> 4) << 16;
+    d |= static_cast<uint64_t>(1024 >> 4) << 32;
+    d |= static_cast<uint64_t>(1) << 46;
+    d |= static_cast<uint64_t>(2) << 61;
+    return d;
+}
+// D = f32, A and B both f16 or both bf16, M = 128
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t tc_idesc(int n, bool b_columns_contiguous) {
+    const uint32_t fmt = sizeof(T) == 2 && exponent_mask<T>() == 0x7f80u ? 1u : 0u;
+    return (1u << 4) | (fmt << 7) | (fmt << 10) | ((b_columns_contiguous ? 1u : 0u) << 16) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(TC_ROWS >> 4) << 24);
+}
+
+struct TcBars {
+    uint64_t full[TC_SLOTS];                                       // TMA -> value check
+    uint64_t ready[TC_SLOTS];                                      // value check -> MMA
+    uint64_t empty[TC_SLOTS];                                      // MMA -> TMA
+    uint64_t q_full[2];                                            // stream -> MMA: the queries of a piece lie in shared memory
+    uint64_t s_full[2];                                            // MMA -> stream: scores (and every product before them) are done
+    uint64_t p_full[2];                                            // stream -> MMA: weights are in place, output rescaled
+    uint64_t o_full[2];                                            // MMA -> stream: the piece's output is done
+    uint64_t o_free[2];                                            // stream -> MMA: it has been read
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(TC_THREADS, 1)
+attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnTcParams p) {
+    constexpr int TILE = tc_tile_bytes<D>(), BOXES = D / 64, BOX = TC_KEYS * 128;      // a box: 128 rows of 64 columns
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* s_q = smem;                                           // [2] queries
+    uint8_t* s_kv = smem + 2 * TILE;                               // [TC_SLOTS]
+    TcBars& bar = *reinterpret_cast<TcBars*>(s_kv + TC_SLOTS * TILE);
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort_storage, s_odd;
+    __shared__ int s_start[3];
+    __shared__ int64_t s_left;
+    volatile int* s_abort = &s_abort_storage;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < TC_SLOTS; ++s) {
+            mbar_init(&bar.full[s], 1);
+            mbar_init(&bar.ready[s], 2);
+            mbar_init(&bar.empty[s], 1);
+        }
+        for (int x = 0; x < 2; ++x) {
+            mbar_init(&bar.q_full[x], TC_ROWS);
+            mbar_init(&bar.s_full[x], 1);
+            mbar_init(&bar.p_full[x], TC_ROWS);
+            mbar_init(&bar.o_full[x], 1);
+            mbar_init(&bar.o_free[x], TC_ROWS);
+        }
+        s_abort_storage = 0;
+        s_odd = 0;
+        mbar_fence_init();
+    }
+    if (warp == 1) tmem_alloc(&s_tmem, TC_COLS);
+    pdl_launch_dependents();
+    pdl_wait();
+    if (warp == 0) {
+        const TcCuts cuts(tc_total(p), gridDim.x);
+        const int64_t from = cuts.at(blockIdx.x);
+        int b, pair, block;
+        tc_locate(p, from, b, pair, block);
+        if (lane == 0) {
+            s_start[0] = b; s_start[1] = pair; s_start[2] = block;
+            s_left = cuts.at(blockIdx.x + 1) - from;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    TcWalk walk = {s_start[0], s_start[1], s_start[2], s_left};
+    TcPiece c;
+
+    if (warp == 0) {
+        // ================= TMA: tiles in the order in which the products use them =================
+        if (lane == 0) {
+            uint32_t pos = 0;
+            auto load = [&](const CUtensorMap* map, int head, int block) {
+                const uint32_t s = pos % TC_SLOTS;
+                if (!wait_or_abort(&bar.empty[s], ((pos / TC_SLOTS) & 1) ^ 1, s_abort)) return false;
+                mbar_expect_tx(&bar.full[s], TILE);
+#pragma unroll
+                for (int i = 0; i < BOXES; ++i) tma_load_4d(s_kv + s * TILE + i * BOX, map, i * 64, block * TC_KEYS, head, c.b, &bar.full[s]);
+                ++pos;
+                return true;
+            };
+            bool ok = true;
+            while (ok && walk.next(p, c)) {
+                const int item = c.pair * 2, streams = item + 1 < p.items ? 2 : 1;
+                const int head[2] = {item / p.tiles, (item + 1) / p.tiles};
+                const int loads = streams == 2 && head[0] != head[1] ? 2 : 1;         // tiles of each kind and block
+                for (int x = 0; x < loads && ok; ++x) ok = load(&map_k, head[x], c.k0);
+                for (int k = c.k0; k < c.k1 && ok; ++k)
+                    for (int x = 0; x < loads && ok; ++x) {
+                        ok = load(&map_v, head[x], k);
+                        if (ok && k + 1 < c.k1) ok = load(&map_k, head[x], k + 1);
+                    }
+            }
+            // after a wait that ran out: the copies under way must land before the shared memory is someone else's
+            for (uint32_t i = pos < TC_SLOTS ? 0 : pos - TC_SLOTS; *s_abort && i < pos; ++i)
+                mbar_wait_bounded(&bar.full[i % TC_SLOTS], (i / TC_SLOTS) & 1);
+        }
+    } else if (warp == 1) {
+        // ================= MMA =================
+        uint32_t pos = 0;
+        uint32_t n_q[2] = {0, 0}, n_p[2] = {0, 0}, n_o[2] = {0, 0};
+        bool ok = true;
+        auto take = [&](uint32_t& slot) {                          // the next tile of the ring
+            slot = pos % TC_SLOTS;
+            ok = ok && wait_or_abort_warp(&bar.ready[slot], (pos / TC_SLOTS) & 1, s_abort);
+            ++pos;
+        };
+        auto scores = [&](int x, uint32_t slot) {
+            tc_fence_after();
+            if (elect_one_lane()) {
+                const uint64_t qa = umma_desc_sw128(smem_u32(s_q + x * TILE)), kb = umma_desc_sw128(smem_u32(s_kv + slot * TILE));
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    const uint32_t off = ((i / 4) * BOX + (i % 4) * 32) >> 4;
+                    umma_f16_ss(tmem + x * 128, qa + off, kb + off, tc_idesc<T>(TC_KEYS, false), i > 0);
+                }
+                umma_commit(&bar.s_full[x]);
+            }
+            __syncwarp();
+        };
+        auto output = [&](int x, uint32_t slot, bool accumulate) {
+            tc_fence_after();
+            if (elect_one_lane()) {
+                const uint64_t vb = umma_desc_sw128_mn(smem_u32(s_kv + slot * TILE));
+#pragma unroll
+                for (int i = 0; i < TC_KEYS / 16; ++i)
+                    umma_f16_ts(tmem + 256 + x * 128, tmem + x * 128 + i * 8, vb + ((i * 2048) >> 4), tc_idesc<T>(D, true), accumulate || i > 0);
+            }
+            __syncwarp();
+        };
+        auto release = [&](uint32_t slot) {
+            if (elect_one_lane()) umma_commit(&bar.empty[slot]);
+            __syncwarp();
+        };
+        while (ok && walk.next(p, c)) {
+            const int item = c.pair * 2, streams = item + 1 < p.items ? 2 : 1;
+            const bool own = streams == 2 && item / p.tiles != (item + 1) / p.tiles;   // each stream has tiles of its own
+            uint32_t k_slot = 0, v_slot = 0;
+            for (int x = 0; x < streams && ok; ++x) {
+                if (x == 0 || own) take(k_slot);
+                ok = ok && wait_or_abort_warp(&bar.q_full[x], n_q[x]++ & 1, s_abort);
+                if (!ok) break;
+                scores(x, k_slot);
+                if (x == streams - 1 || own) release(k_slot);
+            }
+            for (int k = c.k0; k < c.k1 && ok; ++k) {
+                const bool more = k + 1 < c.k1;
+                for (int x = 0; x < streams && ok; ++x) {
+                    if (x == 0 || own) take(v_slot);
+                    if (k == c.k0) ok = ok && wait_or_abort_warp(&bar.o_free[x], (n_o[x]++ & 1) ^ 1, s_abort);
+                    ok = ok && wait_or_abort_warp(&bar.p_full[x], n_p[x]++ & 1, s_abort);
+                    if (!ok) break;
+                    output(x, v_slot, k > c.k0);
+                    if (x == streams - 1 || own) release(v_slot);
+                    if (more) {
+                        if (x == 0 || own) take(k_slot);
+                        if (!ok) break;
+                        scores(x, k_slot);
+                        if (x == streams - 1 || own) release(k_slot);
+                    } else {
+                        if (elect_one_lane()) umma_commit(&bar.o_full[x]);
+                        __syncwarp();
+                    }
+                }
+            }
+        }
+    } else if (warp < 4) {
+        // ================= values of new tokens and of slots past the end =================
+        uint32_t pos = 0;
+        auto check = [&](bool values, int head, int block) {
+            const uint32_t s = pos % TC_SLOTS;
+            if (!wait_or_abort_warp(&bar.full[s], (pos / TC_SLOTS) & 1, s_abort)) return false;
+            ++pos;
+            const int n0 = block * TC_KEYS;
+            if (values && n0 + TC_KEYS > c.len) {
+                uint8_t* tile = s_kv + s * TILE;
+                const int from = max(0, c.len - n0);
+                bool bad = false;
+                for (int i = from * (D / 8) + (threadIdx.x - 64); i < TC_KEYS * (D / 8); i += 64) {
+                    const int row = i / (D / 8), chunk = i % (D / 8);
+                    uint4* at = reinterpret_cast<uint4*>(tile + chunk / 8 * BOX + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+                    uint4 v = *at;
+                    if (n0 + row >= c.end) {
+                        *at = make_uint4(0, 0, 0, 0);
+                    } else if (any_nonfinite<T>(v.x) || any_nonfinite<T>(v.y) || any_nonfinite<T>(v.z) || any_nonfinite<T>(v.w)) {
+                        bad = true;
+                        *at = make_uint4(finite_only<T>(v.x), finite_only<T>(v.y), finite_only<T>(v.z), finite_only<T>(v.w));
+                    }
+                }
+                if (bad) *reinterpret_cast<volatile int*>(&s_odd) = 1;
+                fence_proxy_async_smem();
+                __threadfence_block();
+                __syncwarp();
+            }
+            if (lane == 0) mbar_arrive(&bar.ready[s]);
+            return true;
+        };
+        bool ok = true;
+        while (ok && walk.next(p, c)) {
+            const int item = c.pair * 2, streams = item + 1 < p.items ? 2 : 1;
+            const int head[2] = {item / p.tiles, (item + 1) / p.tiles};
+            const int loads = streams == 2 && head[0] != head[1] ? 2 : 1;
+            for (int x = 0; x < loads && ok; ++x) ok = check(false, head[x], c.k0);
+            for (int k = c.k0; k < c.k1 && ok; ++k)
+                for (int x = 0; x < loads && ok; ++x) {
+                    ok = check(true, head[x], k);
+                    if (ok && k + 1 < c.k1) ok = check(false, head[x], k + 1);
+                }
+        }
+    } else {
+        // ================= streams: one thread per row =================
+        const int x = (warp - 4) >> 2, row = threadIdx.x - 128 - x * TC_ROWS;
+        const uint32_t quarter = static_cast<uint32_t>((warp & 3) * 32) << 16;        // the TMEM lanes of this warp
+        const uint32_t t_s = tmem + quarter + x * 128, t_o = tmem + quarter + 256 + x * 128;
+        uint32_t n_s = 0, n_o = 0;
+        bool ok = true;
+        while (ok && walk.next(p, c)) {
+            const int item = c.pair * 2 + x;
+            if (item >= p.items) continue;
+            const int h = item / p.tiles, r = (item - h * p.tiles) * TC_ROWS + row;
+            const bool real = r < p.a.rows;
+            const int t = real ? r % p.a.T : 0;
+            {   // queries
+                const T* q = real ? attn_q_row<T>(p.a, c.b, h, r) : nullptr;
+                uint8_t* dst = s_q + x * TILE + row * 128;
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (real) v = *reinterpret_cast<const uint4*>(q + i * 8);
+                    if (p.flip) v.x ^= 0x80008000u, v.y ^= 0x80008000u, v.z ^= 0x80008000u, v.w ^= 0x80008000u;
+                    *reinterpret_cast<uint4*>(dst + i / 8 * BOX + (((i & 7) ^ (row & 7)) << 4)) = v;
+                }
+                fence_proxy_async_smem();
+                mbar_arrive(&bar.q_full[x]);
+            }
+            float m = -INFINITY, l = 0.0f;
+            for (int k = c.k0; k < c.k1; ++k) {
+                if (!wait_or_abort_warp(&bar.s_full[x], n_s++ & 1, s_abort)) { ok = false; break; }
+                tc_fence_after();
+                int v[4][32];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tmem_ld_32x32b_x32(t_s + i * 32, v[i]);
+                tmem_ld_wait();
+                const int n0 = k * TC_KEYS;
+                if (n0 + TC_KEYS > c.len) {                        // new tokens or slots past the end: what is not seen gets -infinity
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t sees = 0;
+#pragma unroll 8
+                        for (int e = 0; e < 32; ++e) {
+                            const int n = n0 + i * 32 + e;
+                            if (n < c.end && attn_sees(p.a, c.b, c.len, t, n)) sees |= 1u << e;
+                        }
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (!((sees >> e) & 1u)) v[i][e] = __float_as_int(-INFINITY);
+                    }
+                    __syncwarp();
+                }
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) top[i] = fmaxf(top[i], __int_as_float(v[i][e]));
+                const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale2;
+                if (__any_sync(0xffffffffu, high > m + TC_LAZY || (m == -INFINITY && high > m))) {
+                    const float m_new = fmaxf(m, high);
+                    const float alpha = m_new == -INFINITY ? 1.0f : exp2_fast(m - m_new);
+                    m = m_new;
+                    l *= alpha;
+                    if (k > c.k0) {                                // every product into the output so far is done: s_full says so
+#pragma unroll 1
+                        for (int i = 0; i < D; i += 32) {
+                            int o[32];
+                            tmem_ld_32x32b_x32(t_o + i, o);
+                            tmem_ld_wait();
+                            uint32_t w[2][16];
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) w[e / 16][e % 16] = __float_as_uint(__int_as_float(o[e]) * alpha);
+                            tmem_st_32x32b_x16(t_o + i, w[0]);
+                            tmem_st_32x32b_x16(t_o + i + 16, w[1]);
+                        }
+                    }
+                }
+                const float ref = m == -INFINITY ? 0.0f : m;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float a = exp2_fast(fmaf(__int_as_float(v[i][2 * e]), p.scale2, -ref));
+                        const float b = exp2_fast(fmaf(__int_as_float(v[i][2 * e + 1]), p.scale2, -ref));
+                        sum[e & 3] += a + b;
+                        w[e] = pack2<T>(a, b);
+                    }
+                    tmem_st_32x32b_x16(t_s + i * 16, w);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_st_wait();
+                tc_fence_before();
+                mbar_arrive(&bar.p_full[x]);
+            }
+            if (!ok || !wait_or_abort_warp(&bar.o_full[x], n_o++ & 1, s_abort)) { ok = false; break; }
+            tc_fence_after();
+            const bool whole = c.whole(), odd = *reinterpret_cast<volatile int*>(&s_odd) != 0;
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const int64_t place = ((static_cast<int64_t>(blockIdx.x) * 2 + (c.k0 > 0 ? 0 : 1)) * 2 + x) * TC_ROWS + row;
+            T* out = real ? attn_out_row<T>(p.a, c.b, h, r) : nullptr;
+            if (!whole && real) p.part_ml[place] = make_float2(m, l);
+#pragma unroll 1
+            for (int i = 0; i < D; i += 32) {
+                int o[32];
+                tmem_ld_32x32b_x32(t_o + i, o);
+                tmem_ld_wait();
+                float f[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) f[e] = l == 0.0f ? 0.0f : __int_as_float(o[e]);
+                if (odd && real) {                                 // infinities and NaN of the new tokens that this row sees
+                    for (int n = max(c.len, c.k0 * TC_KEYS); n < min(c.end, c.k1 * TC_KEYS); ++n) {
+                        if (!attn_sees(p.a, c.b, c.len, t, n)) continue;
+                        const T* val = static_cast<const T*>(p.a.v) + c.b * p.a.vb + h * p.a.vh + n * p.a.vs + i;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            const float y = to_float<T>(val[e]);
+                            if (y - y != 0.0f) f[e] += y;
+                        }
+                    }
+                }
+                if (real && whole) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        uint4 w;
+                        w.x = pack2<T>(f[e] * inv, f[e + 1] * inv); w.y = pack2<T>(f[e + 2] * inv, f[e + 3] * inv);
+                        w.z = pack2<T>(f[e + 4] * inv, f[e + 5] * inv); w.w = pack2<T>(f[e + 6] * inv, f[e + 7] * inv);
+                        *reinterpret_cast<uint4*>(out + i + e) = w;
+                    }
+                } else if (real) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(p.part_o + place * D + i + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+                }
+                __syncwarp();
+            }
+            tc_fence_before();
+            mbar_arrive(&bar.o_free[x]);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, TC_COLS);
+    }
+}
+
+// Adds up the pieces of the pairs that the CTAs' cuts went through: blockIdx.x = the CTA that has such a pair's first
+// piece, blockIdx.y = 16 of its 256 rows, one warp per row.
+constexpr int TJ_THREADS = 128;
+constexpr int TJ_ROWS = 16;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(TJ_THREADS) attn_tc_join_kernel(const __grid_constant__ AttnTcParams p, const int ctas) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int64_t total = tc_total(p);
+    const int i = blockIdx.x;
+    const TcCuts cuts(total, ctas);
+    const int64_t from = cuts.at(i), to = cuts.at(i + 1);
+    int b, pair, block;
+    if (to >= total || to == from) return;
+    tc_locate(p, to, b, pair, block);
+    if (block == 0 || to - block < from) return;                   // the cut lies between pairs, or the pair begins in an earlier CTA
+    const int64_t end = to - block + tc_blocks(p, b);
+    int last = i + 1;                                              // the CTA with the pair's last piece
+    while (cuts.at(last + 1) < end) ++last;
+    for (int row2 = blockIdx.y * TJ_ROWS + warp; row2 < (blockIdx.y + 1) * TJ_ROWS; row2 += TJ_THREADS / 32) {
+        const int x = row2 / TC_ROWS, row = row2 % TC_ROWS, item = pair * 2 + x;
+        if (item >= p.items) return;
+        const int h = item / p.tiles, r = (item - h * p.tiles) * TC_ROWS + row;
+        if (r >= p.a.rows) continue;
+        auto place = [&](int cta) { return ((static_cast<int64_t>(cta) * 2 + (cta == i ? 1 : 0)) * 2 + x) * TC_ROWS + row; };
+        float m = -INFINITY;
+        for (int cta = i; cta <= last; ++cta)
+            if (cuts.at(cta) < cuts.at(cta + 1)) m = fmaxf(m, p.part_ml[place(cta)].x);       // the others have no blocks
+        const float ref = m == -INFINITY ? 0.0f : m;
+        float l = 0.0f, o[D / 32];
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) o[e] = 0.0f;
+        for (int cta = i; cta <= last; ++cta) {
+            if (cuts.at(cta) == cuts.at(cta + 1)) continue;
+            const float2 ml = p.part_ml[place(cta)];
+            if (ml.y == 0.0f) continue;
+            const float w = exp2f(ml.x - ref);
+            l += w * ml.y;
+            const float* src = p.part_o + place(cta) * D + lane * (D / 32);
+#pragma unroll
+            for (int e = 0; e < D / 32; ++e) o[e] = fmaf(w, src[e], o[e]);
+        }
+        T* out = attn_out_row<T>(p.a, b, h, r) + lane * (D / 32);
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) out[e] = from_float<T>(l == 0.0f ? 0.0f : o[e] * inv);
+    }
+}
+
+// ---- host side ----------------------------------------------------------------------------------------------------
+
+// Whether a call's sizes are for this kernel (the workspace goes by them); more than one tile of the kernel for few rows.
+static bool attn_tc_sizes(int64_t H, int64_t Hkv, int64_t T, int64_t D, int dtype, bool want_mass) {
+    return dtype != BT_F32 && (D == 64 || D == 128) && !want_mass && H / Hkv * T > AT_ROWS;
+}
+static size_t attn_tc_bytes(int64_t D) {
+    return static_cast<size_t>(sm_count()) * 4 * TC_ROWS * (static_cast<size_t>(D) * sizeof(float) + sizeof(float2));
+}
+// Whether TMA can read the cache: every row on a 16-byte boundary, no stride that it cannot express.
+static bool attn_tc_ok(const AttnParams& p) {
+    if (!attn_stream_ok(p)) return false;
+    const int64_t sizes[3] = {p.S, p.Hkv, p.B}, ks[3] = {p.ks, p.kh, p.kb}, vs[3] = {p.vs, p.vh, p.vb};
+    for (int i = 0; i < 3; ++i)
+        if (sizes[i] > 1 && (ks[i] <= 0 || vs[i] <= 0 || ks[i] >= (int64_t{1} << 38) || vs[i] >= (int64_t{1} << 38))) return false;
+    for (int i = 0; i < 3; ++i)
+        if (p.ob % 8 != 0 || p.oh % 8 != 0 || p.ot % 8 != 0) return false;
+    return aligned(p.out, 16);
+}
+
+static int encode_cache_map(EncodeTiledFn encode, const void* base, int dtype, const AttnParams& p, int64_t sb, int64_t sh, int64_t ss,
+                            CUtensorMap* map) {
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(p.D), static_cast<cuuint64_t>(p.S), static_cast<cuuint64_t>(p.Hkv), static_cast<cuuint64_t>(p.B)};
+    const int64_t s[3] = {ss, sh, sb};
+    cuuint64_t strides[3];
+    for (int i = 0; i < 3; ++i) strides[i] = dims[i + 1] == 1 ? 16 : static_cast<cuuint64_t>(s[i]) * 2;      // of no meaning for a single one
+    const cuuint32_t box[4] = {64, TC_KEYS, 1, 1}, step[4] = {1, 1, 1, 1};
+    const CUresult cr = encode(map, dtype == BT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base),
+                               dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (cr != CUDA_SUCCESS) {
+        set_error("bt_tree_attention: cuTensorMapEncodeTiled failed with code %d", static_cast<int>(cr));
+        return BT_ERR_CUDA;
+    }
+    return BT_OK;
+}
+
+template <typename T, int D>
+static int launch_attn_tc(const AttnParams& a, int dtype, float scale, void* workspace, void* stream) {
+    EncodeTiledFn encode = get_encode_tiled();
+    if (encode == nullptr) {
+        set_error("bt_tree_attention: cuTensorMapEncodeTiled is not available from the driver");
+        return BT_ERR_CUDA;
+    }
+    CUtensorMap map_k, map_v;
+    if (const int rc = encode_cache_map(encode, a.k, dtype, a, a.kb, a.kh, a.ks, &map_k)) return rc;
+    if (const int rc = encode_cache_map(encode, a.v, dtype, a, a.vb, a.vh, a.vs, &map_v)) return rc;
+    AttnTcParams p = {};
+    p.a = a;
+    p.tiles = ceil_div(a.rows, TC_ROWS);
+    p.items = a.Hkv * p.tiles;
+    p.pairs = ceil_div(p.items, 2);
+    p.flip = scale < 0.0f;
+    p.scale2 = std::max(std::abs(scale) * 1.4426950408889634f, 1e-30f);      // not 0: masked scores are -infinity
+    const int ctas = sm_count();
+    p.part_o = static_cast<float*>(workspace);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<size_t>(ctas) * 4 * TC_ROWS * D);
+    static std::atomic<size_t> granted[BT_MAX_DEVICES];
+    if (const int rc = ensure_dynamic_smem(attn_tc_kernel<T, D>, tc_smem<D>(), granted)) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+    cfg.blockDim = dim3(TC_THREADS);
+    cfg.dynamicSmemBytes = tc_smem<D>();
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    BT_CUDA_OK(cudaLaunchKernelEx(&cfg, attn_tc_kernel<T, D>, map_k, map_v, p));
+    cfg.gridDim = dim3(static_cast<unsigned>(ctas), 2 * TC_ROWS / TJ_ROWS);
+    cfg.blockDim = dim3(TJ_THREADS);
+    cfg.dynamicSmemBytes = 0;
+    BT_CUDA_OK(cudaLaunchKernelEx(&cfg, attn_tc_join_kernel<T, D>, p, ctas));
+    return BT_OK;
+}
+
+static int launch_attn_tc_for(const AttnParams& a, int dtype, float scale, void* workspace, void* stream) {
+    if (dtype == BT_F16) return a.D == 64 ? launch_attn_tc<__half, 64>(a, dtype, scale, workspace, stream) : launch_attn_tc<__half, 128>(a, dtype, scale, workspace, stream);
+    return a.D == 64 ? launch_attn_tc<__nv_bfloat16, 64>(a, dtype, scale, workspace, stream) : launch_attn_tc<__nv_bfloat16, 128>(a, dtype, scale, workspace, stream);
+}
+
+}  // namespace bt

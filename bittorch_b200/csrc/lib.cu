@@ -3,6 +3,7 @@
 // and no relocatable device code is needed.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdlib>
 #include <mutex>
 
@@ -68,6 +69,7 @@ __global__ void wait_timeout_selftest_kernel(int polls) {
 #include "beam_select.cuh"
 #include "cache_attention.cuh"
 #include "cache_attention_stream.cuh"
+#include "cache_attention_tcgen05.cuh"
 #include "cache_evict.cuh"
 #include "cache_reorder.cuh"
 #include "float_planes.cuh"
