@@ -29,27 +29,37 @@ namespace bt {
 constexpr int TC_ROWS = 128;                                       // rows of a tile
 constexpr int TC_KEYS = 128;                                       // slots of a block
 constexpr int TC_SLOTS = 4;                                        // ring of key / value tiles
-constexpr int TC_THREADS = 384;                                    // warps: 0 TMA, 1 MMA, 2-3 values of new tokens, 4-7 and 8-11 the streams
+constexpr int TC_THREADS = 320;                                    // warps: 0 TMA, 1 MMA, 2-5 and 6-9 the streams: up to 200 registers a thread
 constexpr int TC_COLS = 512;                                       // TMEM: S0 at 0, S1 at 128, O0 at 256, O1 at 384
 constexpr float TC_LAZY = 8.0f;                                    // how far (in powers of 2) a score may exceed the reference point
 
 template <int D> __host__ __device__ constexpr int tc_tile_bytes() { return TC_KEYS * D * 2; }
-template <int D> constexpr size_t tc_smem() { return 1024 + static_cast<size_t>(2 + TC_SLOTS) * tc_tile_bytes<D>() + 1024; }
+constexpr int TC_NODES = 128;                                      // trees up to this many nodes have their rows as bits in shared memory
+constexpr int TC_STAGE = 32 * 64;                                  // bytes of a warp's staging buffer: 32 rows x 32 columns
+template <int D> constexpr size_t tc_smem() {
+    return 1024 + static_cast<size_t>(2 + TC_SLOTS) * tc_tile_bytes<D>() + 1024 /*barriers*/ + 2 * TC_NODES * 16 + 8 * TC_STAGE;
+}
 
 struct AttnTcParams {
     AttnParams a;
     int tiles;                                                     // of a head
     int items;                                                     // Hkv * tiles of a sequence
     int pairs;                                                     // pairs of tiles of a sequence
-    float scale2;                                                  // |scale| * log2(e)
-    int flip;                                                      // scale < 0: queries are negated instead
-    float* part_o;                                                 // [CTA][2][stream][128][D]
+    float scale2;                                                  // scale * log2(e), not negative
+    float* part_o;                                                 // [CTA][2][stream][D][128]: rows vary fastest, as the threads do
     float2* part_ml;                                               // [CTA][2][stream][128]
 };
 
 // A piece of one pair's line of blocks
 struct TcPiece {
     int b, pair, k0, k1, blocks, len, end;
+    int streams, own;                                              // tiles of the pair; own: they are of two heads, each with its keys and values
+    uint32_t first;                                                // the piece's first tile in the ring's sequence
+    // The tile of the values that stream x multiplies in block k, in the order of tc_sequence
+    __device__ __forceinline__ uint32_t value_tile(int x, int k) const {
+        const uint32_t j = k - k0;
+        return first + (own ? 2 + 4 * j + (k + 1 < k1 ? 2 * x : x) : 1 + 2 * j);
+    }
     __device__ __forceinline__ bool whole() const { return k0 == 0 && k1 == blocks; }
 };
 __device__ __forceinline__ int tc_blocks(const AttnTcParams& p, int b) { return (attn_end(p.a, attn_len(p.a, b)) + TC_KEYS - 1) / TC_KEYS; }
@@ -99,6 +109,7 @@ struct TcCuts {
 struct TcWalk {
     int b, pair, block;
     int64_t left;
+    uint32_t tiles;                                                // of keys and values so far
     __device__ __forceinline__ bool next(const AttnTcParams& p, TcPiece& c) {
         if (left <= 0 || b >= p.a.B) return false;
         c.b = b; c.pair = pair; c.k0 = block;
@@ -106,6 +117,11 @@ struct TcWalk {
         c.end = attn_end(p.a, c.len);
         c.blocks = (c.end + TC_KEYS - 1) / TC_KEYS;
         c.k1 = static_cast<int>(c.blocks - block < left ? c.blocks : block + left);
+        const int item = pair * 2;
+        c.streams = item + 1 < p.items ? 2 : 1;
+        c.own = c.streams == 2 && item / p.tiles != (item + 1) / p.tiles;
+        c.first = tiles;
+        tiles += (c.own ? 4 : 2) * (c.k1 - c.k0);
         left -= c.k1 - c.k0;
         block = 0;
         if (++pair == p.pairs) pair = 0, ++b;
@@ -119,20 +135,68 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, i
         ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
         : "memory");
 }
-__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+// The products of one step as one instruction sequence (issued one by one, each costs as much to prepare as it runs):
+// STEPS k16 steps with both operands in shared memory, K-major, the second 64 columns `BOX >> 4` further.
+template <int STEPS>
+__device__ __forceinline__ void umma_f16_ss_steps(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+    static_assert(STEPS == 4 || STEPS == 8, "head sizes 64 and 128");
+#define BT_SS(off, pred) "add.s64 ta, %1, " #off ";\n\tadd.s64 tb, %2, " #off ";\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], ta, tb, %3, " pred ";\n\t"
+    if (STEPS == 4)
+        asm volatile("{\n\t.reg .pred p0, p1;\n\t.reg .b64 ta, tb;\n\tsetp.ne.b32 p0, 0, 0;\n\tsetp.eq.b32 p1, 0, 0;\n\t"
+                     BT_SS(0, "p0") BT_SS(2, "p1") BT_SS(4, "p1") BT_SS(6, "p1") "}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p0, p1;\n\t.reg .b64 ta, tb;\n\tsetp.ne.b32 p0, 0, 0;\n\tsetp.eq.b32 p1, 0, 0;\n\t"
+                     BT_SS(0, "p0") BT_SS(2, "p1") BT_SS(4, "p1") BT_SS(6, "p1") BT_SS(1024, "p1") BT_SS(1026, "p1") BT_SS(1028, "p1") BT_SS(1030, "p1") "}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc) : "memory");
+#undef BT_SS
 }
-__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+// Eight k16 steps with A from TMEM (8 words of a row per step) and B with contiguous columns (16 rows of 128 bytes per step)
+__device__ __forceinline__ void umma_f16_ts_steps(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+#define BT_TS(i, pred) "add.u32 ta, %1, " #i " * 8;\n\tadd.s64 tb, %2, " #i " * 128;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [ta], tb, %3, " pred ";\n\t"
+    asm volatile("{\n\t.reg .pred p0, p1;\n\t.reg .b32 ta;\n\t.reg .b64 tb;\n\tsetp.ne.b32 p0, %4, 0;\n\tsetp.eq.b32 p1, 0, 0;\n\t"
+                 BT_TS(0, "p0") BT_TS(1, "p1") BT_TS(2, "p1") BT_TS(3, "p1") BT_TS(4, "p1") BT_TS(5, "p1") BT_TS(6, "p1") BT_TS(7, "p1") "}"
                  ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+#undef BT_TS
 }
 __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&v)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
                  ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
                    "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
 }
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, int (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Which of the 32 slots from n0 on a row of token t sees.  `bits`: the row of the tree, 128 nodes, or NULL where the
+// tree is read itself (more nodes than that).
+__device__ __forceinline__ uint32_t tc_seen_word(const AttnParams& p, int b, int len, int end, int t, int n0, const uint4* bits) {
+    if (n0 + 32 <= len) return ~0u;
+    if (n0 >= end) return 0u;
+    const int node = n0 - len, exist = min(end - n0, 32);          // the first slot's node, negative: committed slots come first
+    const uint32_t there = exist >= 32 ? ~0u : (1u << exist) - 1u;
+    if (p.tree == nullptr) {                                       // slots up to its own
+        const int seen = t + 1 - node;
+        return seen <= 0 ? 0u : seen >= 32 ? there : ((1u << seen) - 1u) & there;
+    }
+    if (bits != nullptr) {
+        const uint4 w = bits[t];
+        const int i = node >> 5;                                   // rounds down
+        auto word = [&](int j) { return j < 0 ? ~0u : j == 0 ? w.x : j == 1 ? w.y : j == 2 ? w.z : j == 3 ? w.w : 0u; };
+        return __funnelshift_r(word(i), word(i + 1), node & 31) & there;
+    }
+    uint32_t seen = 0;
+#pragma unroll 8
+    for (int e = 0; e < 32; ++e)
+        if (e < exist && attn_sees(p, b, len, t, n0 + e)) seen |= 1u << e;
+    return seen;
+}
 
 // Operand whose columns (not the summed dimension) are contiguous, 128-byte swizzle: 64 columns x 8 rows per 1024 bytes,
 // row groups 1024 bytes apart, groups of 64 columns a tile of 128 rows apart
@@ -152,9 +216,11 @@ __device__ __forceinline__ constexpr uint32_t tc_idesc(int n, bool b_columns_con
     return (1u << 4) | (fmt << 7) | (fmt << 10) | ((b_columns_contiguous ? 1u : 0u) << 16) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(TC_ROWS >> 4) << 24);
 }
 
+// Barrier over the 128 threads of a stream
+__device__ __forceinline__ void named_barrier_of_stream(int x) { asm volatile("bar.sync %0, 128;" ::"r"(x + 1) : "memory"); }
+
 struct TcBars {
-    uint64_t full[TC_SLOTS];                                       // TMA -> value check
-    uint64_t ready[TC_SLOTS];                                      // value check -> MMA
+    uint64_t full[TC_SLOTS];                                       // TMA -> MMA
     uint64_t empty[TC_SLOTS];                                      // MMA -> TMA
     uint64_t q_full[2];                                            // stream -> MMA: the queries of a piece lie in shared memory
     uint64_t s_full[2];                                            // MMA -> stream: scores (and every product before them) are done
@@ -166,12 +232,15 @@ struct TcBars {
 template <typename T, int D>
 __global__ void __launch_bounds__(TC_THREADS, 1)
 attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnTcParams p) {
+    static_assert(TC_KEYS * 128 >> 4 == 1024, "umma_f16_ss_steps");
     constexpr int TILE = tc_tile_bytes<D>(), BOXES = D / 64, BOX = TC_KEYS * 128;      // a box: 128 rows of 64 columns
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* s_q = smem;                                           // [2] queries
     uint8_t* s_kv = smem + 2 * TILE;                               // [TC_SLOTS]
     TcBars& bar = *reinterpret_cast<TcBars*>(s_kv + TC_SLOTS * TILE);
+    uint4* s_bits = reinterpret_cast<uint4*>(s_kv + TC_SLOTS * TILE + 1024);           // [2][TC_NODES]
+    uint8_t* s_stage = reinterpret_cast<uint8_t*>(s_bits + 2 * TC_NODES);
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort_storage, s_odd;
     __shared__ int s_start[3];
@@ -182,7 +251,6 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     if (threadIdx.x == 0) {
         for (int s = 0; s < TC_SLOTS; ++s) {
             mbar_init(&bar.full[s], 1);
-            mbar_init(&bar.ready[s], 2);
             mbar_init(&bar.empty[s], 1);
         }
         for (int x = 0; x < 2; ++x) {
@@ -213,7 +281,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
-    TcWalk walk = {s_start[0], s_start[1], s_start[2], s_left};
+    TcWalk walk = {s_start[0], s_start[1], s_start[2], s_left, 0};
     TcPiece c;
 
     if (warp == 0) {
@@ -231,9 +299,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             };
             bool ok = true;
             while (ok && walk.next(p, c)) {
-                const int item = c.pair * 2, streams = item + 1 < p.items ? 2 : 1;
+                const int item = c.pair * 2, loads = c.own ? 2 : 1;                    // tiles of each kind and block
                 const int head[2] = {item / p.tiles, (item + 1) / p.tiles};
-                const int loads = streams == 2 && head[0] != head[1] ? 2 : 1;         // tiles of each kind and block
                 for (int x = 0; x < loads && ok; ++x) ok = load(&map_k, head[x], c.k0);
                 for (int k = c.k0; k < c.k1 && ok; ++k)
                     for (int x = 0; x < loads && ok; ++x) {
@@ -248,34 +315,26 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     } else if (warp == 1) {
         // ================= MMA =================
         uint32_t pos = 0;
+        const uint64_t q_desc = umma_desc_sw128(smem_u32(s_q)), k_desc = umma_desc_sw128(smem_u32(s_kv)), v_desc = umma_desc_sw128_mn(smem_u32(s_kv));
         uint32_t n_q[2] = {0, 0}, n_p[2] = {0, 0}, n_o[2] = {0, 0};
         bool ok = true;
         auto take = [&](uint32_t& slot) {                          // the next tile of the ring
             slot = pos % TC_SLOTS;
-            ok = ok && wait_or_abort_warp(&bar.ready[slot], (pos / TC_SLOTS) & 1, s_abort);
+            ok = ok && wait_or_abort_warp(&bar.full[slot], (pos / TC_SLOTS) & 1, s_abort);
             ++pos;
         };
         auto scores = [&](int x, uint32_t slot) {
             tc_fence_after();
             if (elect_one_lane()) {
-                const uint64_t qa = umma_desc_sw128(smem_u32(s_q + x * TILE)), kb = umma_desc_sw128(smem_u32(s_kv + slot * TILE));
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
-                    const uint32_t off = ((i / 4) * BOX + (i % 4) * 32) >> 4;
-                    umma_f16_ss(tmem + x * 128, qa + off, kb + off, tc_idesc<T>(TC_KEYS, false), i > 0);
-                }
+                umma_f16_ss_steps<D / 16>(tmem + x * 128, q_desc + x * (TILE >> 4), k_desc + slot * (TILE >> 4), tc_idesc<T>(TC_KEYS, false));
                 umma_commit(&bar.s_full[x]);
             }
             __syncwarp();
         };
         auto output = [&](int x, uint32_t slot, bool accumulate) {
             tc_fence_after();
-            if (elect_one_lane()) {
-                const uint64_t vb = umma_desc_sw128_mn(smem_u32(s_kv + slot * TILE));
-#pragma unroll
-                for (int i = 0; i < TC_KEYS / 16; ++i)
-                    umma_f16_ts(tmem + 256 + x * 128, tmem + x * 128 + i * 8, vb + ((i * 2048) >> 4), tc_idesc<T>(D, true), accumulate || i > 0);
-            }
+            if (elect_one_lane())
+                umma_f16_ts_steps(tmem + 256 + x * 128, tmem + x * 128, v_desc + slot * (TILE >> 4), tc_idesc<T>(D, true), accumulate);
             __syncwarp();
         };
         auto release = [&](uint32_t slot) {
@@ -283,8 +342,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             __syncwarp();
         };
         while (ok && walk.next(p, c)) {
-            const int item = c.pair * 2, streams = item + 1 < p.items ? 2 : 1;
-            const bool own = streams == 2 && item / p.tiles != (item + 1) / p.tiles;   // each stream has tiles of its own
+            const int streams = c.streams;
+            const bool own = c.own;
             uint32_t k_slot = 0, v_slot = 0;
             for (int x = 0; x < streams && ok; ++x) {
                 if (x == 0 || own) take(k_slot);
@@ -314,121 +373,114 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 }
             }
         }
-    } else if (warp < 4) {
-        // ================= values of new tokens and of slots past the end =================
-        uint32_t pos = 0;
-        auto check = [&](bool values, int head, int block) {
-            const uint32_t s = pos % TC_SLOTS;
-            if (!wait_or_abort_warp(&bar.full[s], (pos / TC_SLOTS) & 1, s_abort)) return false;
-            ++pos;
-            const int n0 = block * TC_KEYS;
-            if (values && n0 + TC_KEYS > c.len) {
-                uint8_t* tile = s_kv + s * TILE;
-                const int from = max(0, c.len - n0);
-                bool bad = false;
-                for (int i = from * (D / 8) + (threadIdx.x - 64); i < TC_KEYS * (D / 8); i += 64) {
-                    const int row = i / (D / 8), chunk = i % (D / 8);
-                    uint4* at = reinterpret_cast<uint4*>(tile + chunk / 8 * BOX + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
-                    uint4 v = *at;
-                    if (n0 + row >= c.end) {
-                        *at = make_uint4(0, 0, 0, 0);
-                    } else if (any_nonfinite<T>(v.x) || any_nonfinite<T>(v.y) || any_nonfinite<T>(v.z) || any_nonfinite<T>(v.w)) {
-                        bad = true;
-                        *at = make_uint4(finite_only<T>(v.x), finite_only<T>(v.y), finite_only<T>(v.z), finite_only<T>(v.w));
-                    }
-                }
-                if (bad) *reinterpret_cast<volatile int*>(&s_odd) = 1;
-                fence_proxy_async_smem();
-                __threadfence_block();
-                __syncwarp();
-            }
-            if (lane == 0) mbar_arrive(&bar.ready[s]);
-            return true;
-        };
-        bool ok = true;
-        while (ok && walk.next(p, c)) {
-            const int item = c.pair * 2, streams = item + 1 < p.items ? 2 : 1;
-            const int head[2] = {item / p.tiles, (item + 1) / p.tiles};
-            const int loads = streams == 2 && head[0] != head[1] ? 2 : 1;
-            for (int x = 0; x < loads && ok; ++x) ok = check(false, head[x], c.k0);
-            for (int k = c.k0; k < c.k1 && ok; ++k)
-                for (int x = 0; x < loads && ok; ++x) {
-                    ok = check(true, head[x], k);
-                    if (ok && k + 1 < c.k1) ok = check(false, head[x], k + 1);
-                }
-        }
     } else {
         // ================= streams: one thread per row =================
-        const int x = (warp - 4) >> 2, row = threadIdx.x - 128 - x * TC_ROWS;
-        const uint32_t quarter = static_cast<uint32_t>((warp & 3) * 32) << 16;        // the TMEM lanes of this warp
+        const int x = (warp - 2) >> 2, row = (warp & 3) * 32 + lane;   // a warp can reach the TMEM lanes of its number mod 4
+        const uint32_t quarter = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t t_s = tmem + quarter + x * 128, t_o = tmem + quarter + 256 + x * 128;
         uint32_t n_s = 0, n_o = 0;
         bool ok = true;
-        while (ok && walk.next(p, c)) {
-            const int item = c.pair * 2 + x;
-            if (item >= p.items) continue;
-            const int h = item / p.tiles, r = (item - h * p.tiles) * TC_ROWS + row;
+        uint8_t* stage = s_stage + (warp - 2) * TC_STAGE;
+        uint4* bits = s_bits + x * TC_NODES;
+        // Copies the queries of a piece's tile, asynchronously: each warp its own 32 rows, neighbouring lanes a row.
+        auto fetch_queries = [&](const TcPiece& w) {
+            constexpr int LANES = D / 8, PER = 32 / LANES;          // lanes of a row, rows at a time
+            const int item = w.pair * 2 + x, h = item / p.tiles, r = (item - h * p.tiles) * TC_ROWS + row;
+            const long long mine = r < p.a.rows ? static_cast<long long>(attn_q_row<T>(p.a, w.b, h, r) - static_cast<const T*>(p.a.q)) : -1;
+            const uint32_t base = smem_u32(s_q + x * TILE);
+            const int chunk = lane % LANES, row0 = row - lane;
+#pragma unroll
+            for (int i = 0; i < 32 / PER; ++i) {
+                const int rr = i * PER + lane / LANES, at = row0 + rr;
+                const long long from = __shfl_sync(0xffffffffu, mine, rr);
+                cp_async16(base + chunk / 8 * BOX + at * 128 + (((chunk & 7) ^ (at & 7)) << 4), static_cast<const T*>(p.a.q) + (from < 0 ? 0 : from) + chunk * 8, from >= 0);
+            }
+            cp_async_commit();
+        };
+        auto queries_there = [&]() {
+            cp_async_wait<0>();
+            fence_proxy_async_smem();
+            mbar_arrive(&bar.q_full[x]);
+        };
+        TcPiece next;
+        auto advance = [&]() {                                     // to the next piece that has a tile for this stream
+            while (walk.next(p, next))
+                if (next.pair * 2 + x < p.items) return true;
+            return false;
+        };
+        bool more = advance();
+        if (more) {
+            fetch_queries(next);
+            queries_there();
+        }
+        while (ok && more) {
+            c = next;
+            const int item = c.pair * 2 + x, h = item / p.tiles, r = (item - h * p.tiles) * TC_ROWS + row;
             const bool real = r < p.a.rows;
             const int t = real ? r % p.a.T : 0;
-            {   // queries
-                const T* q = real ? attn_q_row<T>(p.a, c.b, h, r) : nullptr;
-                uint8_t* dst = s_q + x * TILE + row * 128;
+            const bool table = p.a.tree != nullptr && p.a.T <= TC_NODES;
+            if (table && c.k1 * TC_KEYS > c.len) {                 // this piece reaches the new tokens: a tree row as 128 bits
+                const uint8_t* tree = p.a.tree + c.b * p.a.tree_sb;
+                named_barrier_of_stream(x);                        // the last piece's bits are no longer needed
+#pragma unroll 4
+                for (int i = row >> 5; i < p.a.T; i += 4) {
+                    uint32_t w[4];
 #pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (real) v = *reinterpret_cast<const uint4*>(q + i * 8);
-                    if (p.flip) v.x ^= 0x80008000u, v.y ^= 0x80008000u, v.z ^= 0x80008000u, v.w ^= 0x80008000u;
-                    *reinterpret_cast<uint4*>(dst + i / 8 * BOX + (((i & 7) ^ (row & 7)) << 4)) = v;
+                    for (int j = 0; j < 4; ++j) {
+                        const int node = j * 32 + lane;
+                        w[j] = __ballot_sync(0xffffffffu, node < p.a.T && tree[static_cast<int64_t>(i) * p.a.T + (node < p.a.T ? node : 0)] != 0);
+                    }
+                    if (lane == 0) bits[i] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
-                fence_proxy_async_smem();
-                mbar_arrive(&bar.q_full[x]);
+                named_barrier_of_stream(x);
             }
             float m = -INFINITY, l = 0.0f;
             for (int k = c.k0; k < c.k1; ++k) {
                 if (!wait_or_abort_warp(&bar.s_full[x], n_s++ & 1, s_abort)) { ok = false; break; }
                 tc_fence_after();
-                int v[4][32];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) tmem_ld_32x32b_x32(t_s + i * 32, v[i]);
-                tmem_ld_wait();
+                if (k + 1 == c.k1) {                               // the last product with these queries is done
+                    more = advance();
+                    if (more) fetch_queries(next);
+                }
                 const int n0 = k * TC_KEYS;
-                if (n0 + TC_KEYS > c.len) {                        // new tokens or slots past the end: what is not seen gets -infinity
+                const bool tail = n0 + TC_KEYS > c.len;            // new tokens or slots past the end: what is not seen counts as -infinity
+                uint32_t sees[4] = {~0u, ~0u, ~0u, ~0u};
+                if (tail) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t sees = 0;
-#pragma unroll 8
-                        for (int e = 0; e < 32; ++e) {
-                            const int n = n0 + i * 32 + e;
-                            if (n < c.end && attn_sees(p.a, c.b, c.len, t, n)) sees |= 1u << e;
-                        }
+                    for (int i = 0; i < 4; ++i) sees[i] = tc_seen_word(p.a, c.b, c.len, c.end, t, n0 + i * 32, table ? bits : nullptr);
+                    __syncwarp();
+                }
+                int s[4][32];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tmem_ld_32x32b_x32(t_s + i * 32, s[i]);
+                tmem_ld_wait();
+                if (tail) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
-                            if (!((sees >> e) & 1u)) v[i][e] = __float_as_int(-INFINITY);
-                    }
-                    __syncwarp();
+                            if (!((sees[i] >> e) & 1u)) s[i][e] = __float_as_int(-INFINITY);
                 }
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
+                for (int e = 0; e < 32; e += 2)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) top[i] = fmaxf(top[i], __int_as_float(v[i][e]));
+                    for (int i = 0; i < 4; ++i) top[i] = fmaxf(top[i], fmaxf(__int_as_float(s[i][e]), __int_as_float(s[i][e + 1])));
                 const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale2;
-                if (__any_sync(0xffffffffu, high > m + TC_LAZY || (m == -INFINITY && high > m))) {
-                    const float m_new = fmaxf(m, high);
-                    const float alpha = m_new == -INFINITY ? 1.0f : exp2_fast(m - m_new);
+                if (__any_sync(0xffffffffu, high > m + TC_LAZY)) {
+                    const float m_new = fmaxf(m, high), alpha = m_new == -INFINITY ? 1.0f : exp2_fast(m - m_new);
                     m = m_new;
                     l *= alpha;
                     if (k > c.k0) {                                // every product into the output so far is done: s_full says so
 #pragma unroll 1
-                        for (int i = 0; i < D; i += 32) {
-                            int o[32];
-                            tmem_ld_32x32b_x32(t_o + i, o);
+                        for (int i = 0; i < D; i += 16) {
+                            int o[16];
+                            tmem_ld_32x32b_x16(t_o + i, o);
                             tmem_ld_wait();
-                            uint32_t w[2][16];
+                            uint32_t f[16];
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) w[e / 16][e % 16] = __float_as_uint(__int_as_float(o[e]) * alpha);
-                            tmem_st_32x32b_x16(t_o + i, w[0]);
-                            tmem_st_32x32b_x16(t_o + i + 16, w[1]);
+                            for (int e = 0; e < 16; ++e) f[e] = __float_as_uint(__int_as_float(o[e]) * alpha);
+                            tmem_st_32x32b_x16(t_o + i, f);
                         }
                     }
                 }
@@ -439,25 +491,45 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     uint32_t w[16];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        const float a = exp2_fast(fmaf(__int_as_float(v[i][2 * e]), p.scale2, -ref));
-                        const float b = exp2_fast(fmaf(__int_as_float(v[i][2 * e + 1]), p.scale2, -ref));
+                        const float a = exp2_fast(fmaf(__int_as_float(s[i][2 * e]), p.scale2, -ref));
+                        const float b = exp2_fast(fmaf(__int_as_float(s[i][2 * e + 1]), p.scale2, -ref));
                         sum[e & 3] += a + b;
                         w[e] = pack2<T>(a, b);
                     }
                     tmem_st_32x32b_x16(t_s + i * 16, w);
                 }
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                if (tail && (c.own || x == 0)) {                   // the values of this block, before anything is multiplied by them
+                    const uint32_t tile = c.value_tile(x, k), slot = tile % TC_SLOTS;
+                    if (!wait_or_abort_warp(&bar.full[slot], (tile / TC_SLOTS) & 1, s_abort)) { ok = false; break; }
+                    bool bad = false;
+                    for (int i = max(0, c.len - n0) * (D / 8) + row; i < TC_KEYS * (D / 8); i += TC_ROWS) {
+                        const int n = i / (D / 8), chunk = i % (D / 8);
+                        uint4* at = reinterpret_cast<uint4*>(s_kv + slot * TILE + chunk / 8 * BOX + n * 128 + (((chunk & 7) ^ (n & 7)) << 4));
+                        const uint4 v = *at;
+                        if (n0 + n >= c.end) {
+                            *at = make_uint4(0, 0, 0, 0);
+                        } else if (any_nonfinite<T>(v.x) || any_nonfinite<T>(v.y) || any_nonfinite<T>(v.z) || any_nonfinite<T>(v.w)) {
+                            bad = true;
+                            *at = make_uint4(finite_only<T>(v.x), finite_only<T>(v.y), finite_only<T>(v.z), finite_only<T>(v.w));
+                        }
+                    }
+                    if (bad) *reinterpret_cast<volatile int*>(&s_odd) = 1;
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                }
                 tmem_st_wait();
                 tc_fence_before();
                 mbar_arrive(&bar.p_full[x]);
             }
+            if (ok && more) queries_there();
             if (!ok || !wait_or_abort_warp(&bar.o_full[x], n_o++ & 1, s_abort)) { ok = false; break; }
             tc_fence_after();
             const bool whole = c.whole(), odd = *reinterpret_cast<volatile int*>(&s_odd) != 0;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            const int64_t place = ((static_cast<int64_t>(blockIdx.x) * 2 + (c.k0 > 0 ? 0 : 1)) * 2 + x) * TC_ROWS + row;
-            T* out = real ? attn_out_row<T>(p.a, c.b, h, r) : nullptr;
-            if (!whole && real) p.part_ml[place] = make_float2(m, l);
+            const int64_t place = (static_cast<int64_t>(blockIdx.x) * 2 + (c.k0 > 0 ? 0 : 1)) * 2 + x;
+            const long long out_row = real ? static_cast<long long>(attn_out_row<T>(p.a, c.b, h, r) - static_cast<T*>(p.a.out)) : -1;
+            if (!whole) p.part_ml[place * TC_ROWS + row] = make_float2(m, l);
 #pragma unroll 1
             for (int i = 0; i < D; i += 32) {
                 int o[32];
@@ -477,19 +549,29 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                         }
                     }
                 }
-                if (real && whole) {
+                __syncwarp();
+                if (whole) {                                       // through the warp's buffer, so that four lanes write 64 bytes of a row
 #pragma unroll
                     for (int e = 0; e < 32; e += 8) {
-                        uint4 w;
-                        w.x = pack2<T>(f[e] * inv, f[e + 1] * inv); w.y = pack2<T>(f[e + 2] * inv, f[e + 3] * inv);
-                        w.z = pack2<T>(f[e + 4] * inv, f[e + 5] * inv); w.w = pack2<T>(f[e + 6] * inv, f[e + 7] * inv);
-                        *reinterpret_cast<uint4*>(out + i + e) = w;
+                        uint4 y;
+                        y.x = pack2<T>(f[e] * inv, f[e + 1] * inv); y.y = pack2<T>(f[e + 2] * inv, f[e + 3] * inv);
+                        y.z = pack2<T>(f[e + 4] * inv, f[e + 5] * inv); y.w = pack2<T>(f[e + 6] * inv, f[e + 7] * inv);
+                        *reinterpret_cast<uint4*>(stage + lane * 64 + (((e >> 3) ^ ((lane >> 1) & 3)) << 4)) = y;
                     }
-                } else if (real) {
+                    __syncwarp();
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(p.part_o + place * D + i + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+                    for (int j = 0; j < 4; ++j) {
+                        const int rr = j * 8 + (lane >> 2), q = lane & 3;
+                        const uint4 y = *reinterpret_cast<const uint4*>(stage + rr * 64 + ((q ^ ((rr >> 1) & 3)) << 4));
+                        const long long to = __shfl_sync(0xffffffffu, out_row, rr);
+                        if (to >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(p.a.out) + to + i + q * 8) = y;
+                    }
+                    __syncwarp();
+                } else {
+                    float* to = p.part_o + (place * D + i) * TC_ROWS + row;
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) to[e * TC_ROWS] = f[e];
                 }
-                __syncwarp();
             }
             tc_fence_before();
             mbar_arrive(&bar.o_free[x]);
@@ -504,13 +586,12 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
 }
 
 // Adds up the pieces of the pairs that the CTAs' cuts went through: blockIdx.x = the CTA that has such a pair's first
-// piece, blockIdx.y = 16 of its 256 rows, one warp per row.
-constexpr int TJ_THREADS = 128;
-constexpr int TJ_ROWS = 16;
+// piece, blockIdx.y = the stream and 16 columns; one thread per row, as the pieces were written.
+constexpr int TJ_COLS = 16;
 
 template <typename T, int D>
-__global__ void __launch_bounds__(TJ_THREADS) attn_tc_join_kernel(const __grid_constant__ AttnTcParams p, const int ctas) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+__global__ void __launch_bounds__(TC_ROWS) attn_tc_join_kernel(const __grid_constant__ AttnTcParams p, const int ctas) {
+    const int row = threadIdx.x, x = blockIdx.y / (D / TJ_COLS), d0 = blockIdx.y % (D / TJ_COLS) * TJ_COLS;
     pdl_launch_dependents();
     pdl_wait();
     const int64_t total = tc_total(p);
@@ -524,34 +605,39 @@ __global__ void __launch_bounds__(TJ_THREADS) attn_tc_join_kernel(const __grid_c
     const int64_t end = to - block + tc_blocks(p, b);
     int last = i + 1;                                              // the CTA with the pair's last piece
     while (cuts.at(last + 1) < end) ++last;
-    for (int row2 = blockIdx.y * TJ_ROWS + warp; row2 < (blockIdx.y + 1) * TJ_ROWS; row2 += TJ_THREADS / 32) {
-        const int x = row2 / TC_ROWS, row = row2 % TC_ROWS, item = pair * 2 + x;
-        if (item >= p.items) return;
-        const int h = item / p.tiles, r = (item - h * p.tiles) * TC_ROWS + row;
-        if (r >= p.a.rows) continue;
-        auto place = [&](int cta) { return ((static_cast<int64_t>(cta) * 2 + (cta == i ? 1 : 0)) * 2 + x) * TC_ROWS + row; };
-        float m = -INFINITY;
-        for (int cta = i; cta <= last; ++cta)
-            if (cuts.at(cta) < cuts.at(cta + 1)) m = fmaxf(m, p.part_ml[place(cta)].x);       // the others have no blocks
-        const float ref = m == -INFINITY ? 0.0f : m;
-        float l = 0.0f, o[D / 32];
+    const int item = pair * 2 + x;
+    if (item >= p.items) return;
+    const int h = item / p.tiles, r = (item - h * p.tiles) * TC_ROWS + row;
+    auto place = [&](int cta) { return (static_cast<int64_t>(cta) * 2 + (cta == i ? 1 : 0)) * 2 + x; };
+    auto there = [&](int cta) { return cuts.each > 0 || cuts.at(cta) < cuts.at(cta + 1); };      // a CTA may have no blocks at all
+    float m = -INFINITY;
+#pragma unroll 4
+    for (int cta = i; cta <= last; ++cta)
+        if (there(cta)) m = fmaxf(m, p.part_ml[place(cta) * TC_ROWS + row].x);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f, o[TJ_COLS];
 #pragma unroll
-        for (int e = 0; e < D / 32; ++e) o[e] = 0.0f;
-        for (int cta = i; cta <= last; ++cta) {
-            if (cuts.at(cta) == cuts.at(cta + 1)) continue;
-            const float2 ml = p.part_ml[place(cta)];
-            if (ml.y == 0.0f) continue;
-            const float w = exp2f(ml.x - ref);
-            l += w * ml.y;
-            const float* src = p.part_o + place(cta) * D + lane * (D / 32);
+    for (int e = 0; e < TJ_COLS; ++e) o[e] = 0.0f;
+    for (int cta = i; cta <= last; ++cta) {
+        if (!there(cta)) continue;
+        const float2 ml = p.part_ml[place(cta) * TC_ROWS + row];
+        const float* src = p.part_o + (place(cta) * D + d0) * TC_ROWS + row;
+        float v[TJ_COLS];
 #pragma unroll
-            for (int e = 0; e < D / 32; ++e) o[e] = fmaf(w, src[e], o[e]);
-        }
-        T* out = attn_out_row<T>(p.a, b, h, r) + lane * (D / 32);
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        for (int e = 0; e < TJ_COLS; ++e) v[e] = src[e * TC_ROWS];
+        const float w = ml.y == 0.0f ? 0.0f : exp2f(ml.x - ref);
+        l += w * ml.y;
 #pragma unroll
-        for (int e = 0; e < D / 32; ++e) out[e] = from_float<T>(l == 0.0f ? 0.0f : o[e] * inv);
+        for (int e = 0; e < TJ_COLS; ++e) o[e] = ml.y == 0.0f ? o[e] : fmaf(w, v[e], o[e]);
     }
+    if (r >= p.a.rows) return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint32_t packed[TJ_COLS / 2];
+#pragma unroll
+    for (int e = 0; e < TJ_COLS; e += 2) packed[e / 2] = pack2<T>(l == 0.0f ? 0.0f : o[e] * inv, l == 0.0f ? 0.0f : o[e + 1] * inv);
+    uint4* out = reinterpret_cast<uint4*>(attn_out_row<T>(p.a, b, h, r) + d0);
+    out[0] = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+    out[1] = make_uint4(packed[4], packed[5], packed[6], packed[7]);
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------------
@@ -565,7 +651,7 @@ static size_t attn_tc_bytes(int64_t D) {
 }
 // Whether TMA can read the cache: every row on a 16-byte boundary, no stride that it cannot express.
 static bool attn_tc_ok(const AttnParams& p) {
-    if (!attn_stream_ok(p)) return false;
+    if (!attn_stream_ok(p) || p.scale2 < 0.0f) return false;       // a row's largest score would be its smallest product
     const int64_t sizes[3] = {p.S, p.Hkv, p.B}, ks[3] = {p.ks, p.kh, p.kb}, vs[3] = {p.vs, p.vh, p.vb};
     for (int i = 0; i < 3; ++i)
         if (sizes[i] > 1 && (ks[i] <= 0 || vs[i] <= 0 || ks[i] >= (int64_t{1} << 38) || vs[i] >= (int64_t{1} << 38))) return false;
@@ -606,8 +692,7 @@ static int launch_attn_tc(const AttnParams& a, int dtype, float scale, void* wor
     p.tiles = ceil_div(a.rows, TC_ROWS);
     p.items = a.Hkv * p.tiles;
     p.pairs = ceil_div(p.items, 2);
-    p.flip = scale < 0.0f;
-    p.scale2 = std::max(std::abs(scale) * 1.4426950408889634f, 1e-30f);      // not 0: masked scores are -infinity
+    p.scale2 = std::max(scale * 1.4426950408889634f, 1e-30f);      // not 0: masked scores are -infinity
     const int ctas = sm_count();
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<size_t>(ctas) * 4 * TC_ROWS * D);
@@ -624,8 +709,8 @@ static int launch_attn_tc(const AttnParams& a, int dtype, float scale, void* wor
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
     BT_CUDA_OK(cudaLaunchKernelEx(&cfg, attn_tc_kernel<T, D>, map_k, map_v, p));
-    cfg.gridDim = dim3(static_cast<unsigned>(ctas), 2 * TC_ROWS / TJ_ROWS);
-    cfg.blockDim = dim3(TJ_THREADS);
+    cfg.gridDim = dim3(static_cast<unsigned>(ctas), 2 * D / TJ_COLS);
+    cfg.blockDim = dim3(TC_ROWS);
     cfg.dynamicSmemBytes = 0;
     BT_CUDA_OK(cudaLaunchKernelEx(&cfg, attn_tc_join_kernel<T, D>, p, ctas));
     return BT_OK;
