@@ -340,7 +340,8 @@ def beam_select(logits: Tensor, scores: Tensor, select: Optional[int], finished:
         finished = finished.contiguous()
     dev, b = logits.device, head[1]
     out = torch.empty((b, n), dtype=torch.float32, device=dev)
-    tokens, parents = torch.empty((2, b, n), dtype=torch.int64, device=dev).unbind()
+    tokens = torch.empty((b, n), dtype=torch.int64, device=dev)
+    parents = torch.empty((b, n), dtype=torch.int64, device=dev)
     work = torch.empty(need, dtype=torch.uint8, device=dev)
     _call(index, _beam_select, logits.data_ptr(), *head, scores.data_ptr(), None if finished is None else finished.data_ptr(),
           0 if end_token is None else end_token, n, out.data_ptr(), tokens.data_ptr(), parents.data_ptr(), work.data_ptr(), need)

@@ -4,7 +4,7 @@
 // one piece of a row, held in registers, and leaves the piece's maximum, its sum of exponentials and its n largest
 // logits; beam_join makes the log-sums and ranks the survivors of all beams in float64.  Bound by HBM (the logits).
 //
-// The n largest of a piece: 64 groups of four threads have a maximum each, and the n-th of those (n <= 64) bounds the
+// The n largest of a piece: 16 or 64 groups of threads have a maximum each, and the n-th of those bounds the
 // n-th of the piece from below.  What is not below it is collected and ranked by counting: with independent logits a
 // little more than n.  A logit and its place make one 64-bit key (larger logit first, then the lower place), so that no
 // two are equal.  A plateau of equal logits can pass the bound in any number; a list that overflows is abandoned for n
@@ -12,7 +12,8 @@
 //
 // A row's elements go to threads by their place in the row, whatever the row's alignment (a misaligned row is read in
 // aligned 16-byte words and shifted): equal rows have equal sums, so that ties between beams are ties.  Exponentials
-// are float32 (2^-22), their sums float32 within a thread (32 terms) and float64 from there.
+// are float32 (2^-22) and so are their sums within a warp (1024 terms, each a tree of at most 10 roundings), float64 from
+// there: a log-sum is off by about 1e-8.
 #pragma once
 
 #include "cache_common.cuh"
@@ -23,8 +24,10 @@ namespace bt {
 constexpr int BS_THREADS = 256;
 constexpr int BS_WARPS = BS_THREADS / 32;
 constexpr int BS_WORDS = 4;                                        // 16-byte words of a thread
-constexpr int BS_GROUPS = BS_THREADS / 4;                          // at least BT_BEAM_MAX_SELECT
 constexpr int BS_LIST = 1024;
+// Groups of neighbouring threads whose maxima bound the n-th largest of a piece: at least n, and as few as that allows,
+// since all are compared with all.
+constexpr int BS_FEW_GROUPS = 16, BS_GROUPS = 64;
 static_assert(BS_GROUPS >= BT_BEAM_MAX_SELECT, "the n-th group maximum must exist");
 template <typename T> __host__ __device__ constexpr int bs_per_word() { return 16 / static_cast<int>(sizeof(T)); }
 template <typename T> __host__ __device__ constexpr int bs_piece() { return BS_THREADS * BS_WORDS * bs_per_word<T>(); }
@@ -164,12 +167,12 @@ __device__ __forceinline__ unsigned long long logit_key(float x, int64_t v) {
     return (static_cast<unsigned long long>(ordered_key(x != x ? -INFINITY : x)) << 32) | (0xffffffffu - static_cast<uint32_t>(v));
 }
 
-template <typename T>
-__global__ void __launch_bounds__(BS_THREADS, 8) beam_scan_kernel(const BeamParams p) {
+template <typename T, int GROUPS>
+__global__ void __launch_bounds__(BS_THREADS, 6) beam_scan_kernel(const BeamParams p) {
     constexpr int PER = bs_per_word<T>(), PIECE = bs_piece<T>();
     __shared__ unsigned long long s_list[BS_LIST];
-    __shared__ double s_sum[BS_WARPS];
-    __shared__ float s_max[BS_WARPS], s_group[BS_GROUPS];
+    __shared__ float s_sum[BS_WARPS];
+    __shared__ float s_max[BS_WARPS], s_group[GROUPS];
     __shared__ unsigned long long s_best[BS_WARPS];
     __shared__ float s_edge;
     __shared__ int s_count;
@@ -179,9 +182,9 @@ __global__ void __launch_bounds__(BS_THREADS, 8) beam_scan_kernel(const BeamPara
     if (tid == 0) s_count = 0;
     pdl_launch_dependents();
     pdl_wait();
-    if (!beam_live(p, row)) return;                                // for every thread of the CTA; beam_join knows
-    const int64_t b = row / p.W;
-    const T* x0 = static_cast<const T*>(p.logits) + b * p.ld_b + (row - b * p.W) * p.ld_w;
+    const bool live = beam_live(p, row);
+    const int b = static_cast<int>(row) / p.W;
+    const T* x0 = static_cast<const T*>(p.logits) + b * p.ld_b + (static_cast<int>(row) - b * p.W) * p.ld_w;
     const int64_t v0 = static_cast<int64_t>(piece) * PIECE;
     const int64_t w0 = v0 / PER + tid;                             // this thread's first word; the others follow at BS_THREADS
 
@@ -196,28 +199,32 @@ __global__ void __launch_bounds__(BS_THREADS, 8) beam_scan_kernel(const BeamPara
         else if (wi > 0 && (wi + 2) * PER <= p.V) word[i] = shifted_word(words[wi], words[wi + 1], shift);
         else word[i] = row_word_at_end<T>(x0, p.V, wi);
     }
+    if (!live) return;                                             // for every thread of the CTA; beam_join knows
     WordMax<T> top;
 #pragma unroll
     for (int i = 0; i < BS_WORDS; ++i) top.add(word[i]);
     const float mine = top.get();
-    float mx = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    if ((lane & 3) == 0) s_group[tid >> 2] = mx;
+    constexpr int MEMBERS = BS_THREADS / GROUPS;
+    float mx = mine;
+#pragma unroll
+    for (int o = 1; o < MEMBERS; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    if ((lane & (MEMBERS - 1)) == 0) s_group[tid / MEMBERS] = mx;
     mx = warp_max(mx);
     __syncthreads();
-    {   // the n-th largest group maximum: the four threads of a group count the others above it, 16 each
-        const float a = s_group[tid >> 2];
+    {   // the n-th largest group maximum: a group's threads compare it with all, GROUPS / MEMBERS each
+        const float a = s_group[tid / MEMBERS];
         int above = 0, level = 0;
 #pragma unroll
-        for (int i = 0; i < BS_GROUPS / 4; ++i) {
-            const float x = s_group[(tid & 3) * (BS_GROUPS / 4) + i];
+        for (int i = 0; i < GROUPS / MEMBERS; ++i) {
+            const float x = s_group[(tid & (MEMBERS - 1)) * (GROUPS / MEMBERS) + i];
             above += x > a;
             level += x >= a;
         }
-        above += __shfl_xor_sync(0xffffffffu, above, 1);
-        level += __shfl_xor_sync(0xffffffffu, level, 1);
-        above += __shfl_xor_sync(0xffffffffu, above, 2);
-        level += __shfl_xor_sync(0xffffffffu, level, 2);
+#pragma unroll
+        for (int o = 1; o < MEMBERS; o <<= 1) {
+            above += __shfl_xor_sync(0xffffffffu, above, o);
+            level += __shfl_xor_sync(0xffffffffu, level, o);
+        }
         if (above < p.n && level >= p.n) s_edge = a;               // groups that tie here write the same value
     }
     float sum = 0.0f;
@@ -231,9 +238,9 @@ __global__ void __launch_bounds__(BS_THREADS, 8) beam_scan_kernel(const BeamPara
             for (int e = 0; e < PER; ++e) sum += exp2_fast((fmaxf(x[e], -INFINITY) - mx) * 1.4426950408889634f);     // a NaN adds 0
         }
     }
-    const double total = warp_add_double(static_cast<double>(sum));
+    sum = warp_add(sum);
     if (lane == 0) {
-        s_sum[warp] = total;
+        s_sum[warp] = sum;
         s_max[warp] = mx;
     }
     __syncthreads();
@@ -262,7 +269,7 @@ __global__ void __launch_bounds__(BS_THREADS, 8) beam_scan_kernel(const BeamPara
         const float m_w = lane < BS_WARPS ? s_max[lane] : -INFINITY, m = warp_max(m_w);
         double all = 0.0;
         if (lane < BS_WARPS && m - m == 0.0f && s_sum[lane] > 0.0)
-            all = s_sum[lane] * exp2(1.4426950408889634 * (static_cast<double>(m_w) - static_cast<double>(m)));
+            all = static_cast<double>(s_sum[lane]) * exp2(1.4426950408889634 * (static_cast<double>(m_w) - static_cast<double>(m)));
         all = warp_add_double(all);
         if (lane == 0) {
             p.piece_max[row * p.pieces + piece] = m;
@@ -480,6 +487,11 @@ static BeamPlan beam_plan(int64_t B, int64_t W, int64_t V, int dtype, int64_t n)
     a.maxima = up(all * 4);
     return a;
 }
+template <typename T>
+static int launch_beam_scan(const BeamParams& p, dim3 grid, void* stream) {
+    if (p.n <= BS_FEW_GROUPS) return launch_early(beam_scan_kernel<T, BS_FEW_GROUPS>, "beam_scan_kernel", grid, BS_THREADS, 0, stream, p);
+    return launch_early(beam_scan_kernel<T, BS_GROUPS>, "beam_scan_kernel", grid, BS_THREADS, 0, stream, p);
+}
 static bool beam_sizes_ok(int64_t B, int64_t W, int64_t V, int64_t n) {
     return B > 0 && W > 0 && V > 0 && n > 0 && (V >= n || n <= W * V);
 }
@@ -517,9 +529,9 @@ extern "C" int bt_beam_select(const void* logits, int dtype, int64_t B, int64_t 
     p.out_scores = out_scores; p.out_tokens = out_tokens; p.out_parents = out_parents;
     const dim3 grid(static_cast<unsigned>(B * W * plan.pieces));
     int rc;
-    if (dtype == BT_F32) rc = launch_early(beam_scan_kernel<float>, "beam_scan_kernel", grid, BS_THREADS, 0, stream, p);
-    else if (dtype == BT_F16) rc = launch_early(beam_scan_kernel<__half>, "beam_scan_kernel", grid, BS_THREADS, 0, stream, p);
-    else rc = launch_early(beam_scan_kernel<__nv_bfloat16>, "beam_scan_kernel", grid, BS_THREADS, 0, stream, p);
+    if (dtype == BT_F32) rc = launch_beam_scan<float>(p, grid, stream);
+    else if (dtype == BT_F16) rc = launch_beam_scan<__half>(p, grid, stream);
+    else rc = launch_beam_scan<__nv_bfloat16>(p, grid, stream);
     if (rc != BT_OK) return rc;
     return launch_early(beam_join_kernel, "beam_join_kernel", dim3(static_cast<unsigned>(B)), BJ_THREADS, 0, stream, p);
 }

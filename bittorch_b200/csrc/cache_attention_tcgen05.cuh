@@ -29,8 +29,9 @@ namespace bt {
 constexpr int TC_ROWS = 128;                                       // rows of a tile
 constexpr int TC_KEYS = 128;                                       // slots of a block
 constexpr int TC_SLOTS = 4;                                        // ring of key / value tiles
-constexpr int TC_THREADS = 320;                                    // warps: 0 TMA, 1 MMA, 2-5 and 6-9 the streams: up to 200 registers a thread
-constexpr int TC_COLS = 512;                                       // TMEM: S0 at 0, S1 at 128, O0 at 256, O1 at 384
+constexpr int TC_THREADS = 352;                                    // warps: 0 TMA, 1 scores, 10 outputs, 2-5 and 6-9 the streams
+constexpr int TC_COLS = 512;                                       // TMEM: scores at 0, weights at 128 and 192, outputs at 256 and 384
+constexpr int TC_WEIGHTS = 128, TC_OUTPUT = 256;
 constexpr float TC_LAZY = 8.0f;                                    // how far (in powers of 2) a score may exceed the reference point
 
 template <int D> __host__ __device__ constexpr int tc_tile_bytes() { return TC_KEYS * D * 2; }
@@ -55,12 +56,6 @@ struct TcPiece {
     int b, pair, k0, k1, blocks, len, end;
     int streams, own;                                              // tiles of the pair; own: they are of two heads, each with its keys and values
     uint32_t first;                                                // the piece's first tile in the ring's sequence
-    // The tile of the values that stream x multiplies in block k, in the order of tc_sequence
-    __device__ __forceinline__ uint32_t value_tile(int x, int k) const {
-        const uint32_t j = k - k0;
-        return first + (own ? 2 + 4 * j + (k + 1 < k1 ? 2 * x : x) : 1 + 2 * j);
-    }
-    __device__ __forceinline__ bool whole() const { return k0 == 0 && k1 == blocks; }
 };
 __device__ __forceinline__ int tc_blocks(const AttnTcParams& p, int b) { return (attn_end(p.a, attn_len(p.a, b)) + TC_KEYS - 1) / TC_KEYS; }
 
@@ -105,6 +100,20 @@ struct TcCuts {
     __device__ __forceinline__ TcCuts(int64_t total, unsigned n) : each(total / n), rest(static_cast<unsigned>(total % n)), ctas(n) {}
     __device__ __forceinline__ int64_t at(unsigned i) const { return each * i + rest * i / ctas; }
 };
+
+// The place of the values of block j of n, for stream x, in the sequence of a piece's tiles (as the TMA warp brings them)
+__device__ __forceinline__ uint32_t tc_value_tile(bool own, int n, int j, int x) {
+    const int ahead = min(j, max(n - 2, 0));                       // keys of blocks j + 1 that came before
+    if (!own) return min(2, n) + j + ahead;
+    return 2 + (n > 1) + 2 * j + min(j, n - 1) + ahead + (x ? 1 + (j + 1 < n) : 0);
+}
+
+// The same for the keys
+__device__ __forceinline__ uint32_t tc_key_tile(bool own, int n, int j, int x) {
+    if (!own) return j < 2 ? j : tc_value_tile(own, n, j - 2, 0) + 1;
+    if (x == 1) return j == 0 ? 1 : tc_value_tile(own, n, j - 1, 0) + 1;
+    return j < 2 ? 2 * j : tc_value_tile(own, n, j - 2, 1) + 1;
+}
 
 struct TcWalk {
     int b, pair, block;
@@ -172,6 +181,20 @@ __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, int (&v)[16])
         : "r"(taddr)
         : "memory");
 }
+// Two float32 operations in one instruction
+__device__ __forceinline__ float2 fma_f32x2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add_f32x2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Which of the 32 slots from n0 on a row of token t sees.  `bits`: the row of the tree, 128 nodes, or NULL where the
@@ -220,14 +243,32 @@ __device__ __forceinline__ constexpr uint32_t tc_idesc(int n, bool b_columns_con
 __device__ __forceinline__ void named_barrier_of_stream(int x) { asm volatile("bar.sync %0, 128;" ::"r"(x + 1) : "memory"); }
 
 struct TcBars {
-    uint64_t full[TC_SLOTS];                                       // TMA -> MMA
-    uint64_t empty[TC_SLOTS];                                      // MMA -> TMA
-    uint64_t q_full[2];                                            // stream -> MMA: the queries of a piece lie in shared memory
-    uint64_t s_full[2];                                            // MMA -> stream: scores (and every product before them) are done
-    uint64_t p_full[2];                                            // stream -> MMA: weights are in place, output rescaled
-    uint64_t o_full[2];                                            // MMA -> stream: the piece's output is done
-    uint64_t o_free[2];                                            // stream -> MMA: it has been read
+    uint64_t full[TC_SLOTS];                                       // TMA -> products
+    uint64_t empty[TC_SLOTS];                                      // products -> TMA
+    uint64_t q_full[2];                                            // stream -> scores: the queries of a piece lie in shared memory
+    uint64_t s_full[2];                                            // scores -> stream: they are there
+    uint64_t s_read[2];                                            // stream -> scores: they are in registers, the buffer is free
+    uint64_t p_full[2];                                            // stream -> outputs: weights are in place, output rescaled
+    uint64_t v_checked;                                            // first stream -> second: values that both multiply have been looked through
+    uint64_t pv_done[2];                                           // outputs -> stream: they have been multiplied
 };
+
+// Copies the queries of a tile into shared memory, asynchronously: each warp its own 32 rows, neighbouring lanes a row.
+// (A function of its own: it runs once per piece and must not cost the loop over the blocks its registers.)
+template <typename T, int D>
+__device__ __noinline__ void tc_fetch_queries(const AttnTcParams& p, int b, int item, int row, uint32_t base) {
+    constexpr int LANES = D / 8, PER = 32 / LANES, BOX = TC_KEYS * 128;          // lanes of a row, rows at a time
+    const int lane = threadIdx.x & 31, h = item / p.tiles, r = (item - h * p.tiles) * TC_ROWS + row;
+    const long long mine = r < p.a.rows ? static_cast<long long>(attn_q_row<T>(p.a, b, h, r) - static_cast<const T*>(p.a.q)) : -1;
+    const int chunk = lane % LANES, row0 = row - lane;
+#pragma unroll 4
+    for (int i = 0; i < 32 / PER; ++i) {
+        const int rr = i * PER + lane / LANES, at = row0 + rr;
+        const long long from = __shfl_sync(0xffffffffu, mine, rr);
+        cp_async16(base + chunk / 8 * BOX + at * 128 + (((chunk & 7) ^ (at & 7)) << 4), static_cast<const T*>(p.a.q) + (from < 0 ? 0 : from) + chunk * 8, from >= 0);
+    }
+    cp_async_commit();
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(TC_THREADS, 1)
@@ -245,6 +286,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     __shared__ int s_abort_storage, s_odd;
     __shared__ int s_start[3];
     __shared__ int64_t s_left;
+    __shared__ TcWalk s_walk[8];                                   // per warp of the streams
+    __shared__ TcPiece s_piece[8][2];                              // the piece that the warp is in and the one after it
     volatile int* s_abort = &s_abort_storage;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -256,10 +299,11 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         for (int x = 0; x < 2; ++x) {
             mbar_init(&bar.q_full[x], TC_ROWS);
             mbar_init(&bar.s_full[x], 1);
+            mbar_init(&bar.s_read[x], TC_ROWS);
             mbar_init(&bar.p_full[x], TC_ROWS);
-            mbar_init(&bar.o_full[x], 1);
-            mbar_init(&bar.o_free[x], TC_ROWS);
+            mbar_init(&bar.pv_done[x], 1);
         }
+        mbar_init(&bar.v_checked, TC_ROWS);
         s_abort_storage = 0;
         s_odd = 0;
         mbar_fence_init();
@@ -302,119 +346,107 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 const int item = c.pair * 2, loads = c.own ? 2 : 1;                    // tiles of each kind and block
                 const int head[2] = {item / p.tiles, (item + 1) / p.tiles};
                 for (int x = 0; x < loads && ok; ++x) ok = load(&map_k, head[x], c.k0);
-                for (int k = c.k0; k < c.k1 && ok; ++k)
-                    for (int x = 0; x < loads && ok; ++x) {
-                        ok = load(&map_v, head[x], k);
-                        if (ok && k + 1 < c.k1) ok = load(&map_k, head[x], k + 1);
+                if (ok && c.k0 + 1 < c.k1) ok = load(&map_k, head[0], c.k0 + 1);
+                for (int k = c.k0; k < c.k1 && ok; ++k) {
+                    ok = load(&map_v, head[0], k);
+                    if (loads == 2) {
+                        if (ok && k + 1 < c.k1) ok = load(&map_k, head[1], k + 1);
+                        if (ok) ok = load(&map_v, head[1], k);
                     }
+                    if (ok && k + 2 < c.k1) ok = load(&map_k, head[0], k + 2);
+                }
             }
             // after a wait that ran out: the copies under way must land before the shared memory is someone else's
             for (uint32_t i = pos < TC_SLOTS ? 0 : pos - TC_SLOTS; *s_abort && i < pos; ++i)
                 mbar_wait_bounded(&bar.full[i % TC_SLOTS], (i / TC_SLOTS) & 1);
         }
-    } else if (warp == 1) {
-        // ================= MMA =================
-        uint32_t pos = 0;
+    } else if (warp == 1 || warp == 10) {
+        // ================= products: warp 1 the scores of both streams, warp 10 their outputs =================
+        // Two warps, because a product is issued no faster than the tensor cores take it: weights that are ready must not
+        // wait behind scores.  Everything that the products go by is made provably the same in all lanes: the compiler then
+        // keeps descriptors and addresses in uniform registers, where the instruction wants them.
+        const bool values = __shfl_sync(0xffffffffu, warp, 0) == 10;
+        const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
         const uint64_t q_desc = umma_desc_sw128(smem_u32(s_q)), k_desc = umma_desc_sw128(smem_u32(s_kv)), v_desc = umma_desc_sw128_mn(smem_u32(s_kv));
-        uint32_t n_q[2] = {0, 0}, n_p[2] = {0, 0}, n_o[2] = {0, 0};
+        uint32_t n_q[2] = {0, 0}, n_p[2] = {0, 0}, n_read[2] = {0, 0};               // phases
+        int unread = -1;                                           // the stream whose scores the buffer holds
         bool ok = true;
-        auto take = [&](uint32_t& slot) {                          // the next tile of the ring
-            slot = pos % TC_SLOTS;
-            ok = ok && wait_or_abort_warp(&bar.full[slot], (pos / TC_SLOTS) & 1, s_abort);
-            ++pos;
-        };
-        auto scores = [&](int x, uint32_t slot) {
-            tc_fence_after();
-            if (elect_one_lane()) {
-                umma_f16_ss_steps<D / 16>(tmem + x * 128, q_desc + x * (TILE >> 4), k_desc + slot * (TILE >> 4), tc_idesc<T>(TC_KEYS, false));
-                umma_commit(&bar.s_full[x]);
-            }
-            __syncwarp();
-        };
-        auto output = [&](int x, uint32_t slot, bool accumulate) {
-            tc_fence_after();
-            if (elect_one_lane())
-                umma_f16_ts_steps(tmem + 256 + x * 128, tmem + x * 128, v_desc + slot * (TILE >> 4), tc_idesc<T>(D, true), accumulate);
-            __syncwarp();
-        };
-        auto release = [&](uint32_t slot) {
-            if (elect_one_lane()) umma_commit(&bar.empty[slot]);
-            __syncwarp();
-        };
-        while (ok && walk.next(p, c)) {
-            const int streams = c.streams;
-            const bool own = c.own;
-            uint32_t k_slot = 0, v_slot = 0;
-            for (int x = 0; x < streams && ok; ++x) {
-                if (x == 0 || own) take(k_slot);
-                ok = ok && wait_or_abort_warp(&bar.q_full[x], n_q[x]++ & 1, s_abort);
-                if (!ok) break;
-                scores(x, k_slot);
-                if (x == streams - 1 || own) release(k_slot);
-            }
-            for (int k = c.k0; k < c.k1 && ok; ++k) {
-                const bool more = k + 1 < c.k1;
+        auto tile_there = [&](uint32_t tile) { ok = ok && wait_or_abort_warp(&bar.full[tile % TC_SLOTS], (tile / TC_SLOTS) & 1, s_abort); };
+        while (ok && __all_sync(0xffffffffu, walk.next(p, c))) {
+            const int blocks = __shfl_sync(0xffffffffu, c.k1 - c.k0, 0), streams = __shfl_sync(0xffffffffu, c.streams, 0);
+            const bool own = __shfl_sync(0xffffffffu, c.own, 0) != 0;
+            const uint32_t first = __shfl_sync(0xffffffffu, c.first, 0);
+            for (int j = 0; j < blocks && ok; ++j)
                 for (int x = 0; x < streams && ok; ++x) {
-                    if (x == 0 || own) take(v_slot);
-                    if (k == c.k0) ok = ok && wait_or_abort_warp(&bar.o_free[x], (n_o[x]++ & 1) ^ 1, s_abort);
-                    ok = ok && wait_or_abort_warp(&bar.p_full[x], n_p[x]++ & 1, s_abort);
-                    if (!ok) break;
-                    output(x, v_slot, k > c.k0);
-                    if (x == streams - 1 || own) release(v_slot);
-                    if (more) {
-                        if (x == 0 || own) take(k_slot);
+                    const bool last_use = own || x == streams - 1;
+                    if (!values) {
+                        const uint32_t tile = first + tc_key_tile(own, blocks, j, x), slot = tile % TC_SLOTS;
+                        if (x == 0 || own) tile_there(tile);
+                        if (j == 0) ok = ok && wait_or_abort_warp(&bar.q_full[x], n_q[x]++ & 1, s_abort);
+                        if (unread >= 0) ok = ok && wait_or_abort_warp(&bar.s_read[unread], n_read[unread]++ & 1, s_abort);
+                        unread = x;
                         if (!ok) break;
-                        scores(x, k_slot);
-                        if (x == streams - 1 || own) release(k_slot);
+                        tc_fence_after();
+                        if (elect_one_lane()) {
+                            umma_f16_ss_steps<D / 16>(tmem_u, q_desc + x * (TILE >> 4), k_desc + slot * (TILE >> 4), tc_idesc<T>(TC_KEYS, false));
+                            umma_commit(&bar.s_full[x]);
+                            if (last_use) umma_commit(&bar.empty[slot]);
+                        }
                     } else {
-                        if (elect_one_lane()) umma_commit(&bar.o_full[x]);
-                        __syncwarp();
+                        const uint32_t tile = first + tc_value_tile(own, blocks, j, x), slot = tile % TC_SLOTS;
+                        if (x == 0 || own) tile_there(tile);
+                        ok = ok && wait_or_abort_warp(&bar.p_full[x], n_p[x]++ & 1, s_abort);
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (elect_one_lane()) {
+                            umma_f16_ts_steps(tmem_u + TC_OUTPUT + x * 128, tmem_u + TC_WEIGHTS + x * 64, v_desc + slot * (TILE >> 4), tc_idesc<T>(D, true), j > 0);
+                            umma_commit(&bar.pv_done[x]);
+                            if (last_use) umma_commit(&bar.empty[slot]);
+                        }
                     }
+                    __syncwarp();
                 }
-            }
         }
     } else {
         // ================= streams: one thread per row =================
         const int x = (warp - 2) >> 2, row = (warp & 3) * 32 + lane;   // a warp can reach the TMEM lanes of its number mod 4
         const uint32_t quarter = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t t_s = tmem + quarter + x * 128, t_o = tmem + quarter + 256 + x * 128;
-        uint32_t n_s = 0, n_o = 0;
+        const uint32_t t_s = tmem + quarter, t_p = t_s + TC_WEIGHTS + x * 64, t_o = t_s + TC_OUTPUT + x * 128;
+        uint32_t n_s = 0, n_pv = 0, n_checked = 0;
         bool ok = true;
         uint8_t* stage = s_stage + (warp - 2) * TC_STAGE;
         uint4* bits = s_bits + x * TC_NODES;
-        // Copies the queries of a piece's tile, asynchronously: each warp its own 32 rows, neighbouring lanes a row.
-        auto fetch_queries = [&](const TcPiece& w) {
-            constexpr int LANES = D / 8, PER = 32 / LANES;          // lanes of a row, rows at a time
-            const int item = w.pair * 2 + x, h = item / p.tiles, r = (item - h * p.tiles) * TC_ROWS + row;
-            const long long mine = r < p.a.rows ? static_cast<long long>(attn_q_row<T>(p.a, w.b, h, r) - static_cast<const T*>(p.a.q)) : -1;
-            const uint32_t base = smem_u32(s_q + x * TILE);
-            const int chunk = lane % LANES, row0 = row - lane;
-#pragma unroll
-            for (int i = 0; i < 32 / PER; ++i) {
-                const int rr = i * PER + lane / LANES, at = row0 + rr;
-                const long long from = __shfl_sync(0xffffffffu, mine, rr);
-                cp_async16(base + chunk / 8 * BOX + at * 128 + (((chunk & 7) ^ (at & 7)) << 4), static_cast<const T*>(p.a.q) + (from < 0 ? 0 : from) + chunk * 8, from >= 0);
-            }
-            cp_async_commit();
-        };
+        auto fetch_queries = [&](const volatile TcPiece& w) { tc_fetch_queries<T, D>(p, w.b, w.pair * 2 + x, row, smem_u32(s_q + x * TILE)); };
         auto queries_there = [&]() {
             cp_async_wait<0>();
             fence_proxy_async_smem();
             mbar_arrive(&bar.q_full[x]);
         };
-        TcPiece next;
+        int turn = 0;
+        // Where the stream is lives in shared memory: the registers are for the scores.
         auto advance = [&]() {                                     // to the next piece that has a tile for this stream
-            while (walk.next(p, next))
-                if (next.pair * 2 + x < p.items) return true;
-            return false;
+            __syncwarp();
+            if (lane == 0) {
+                TcWalk at = s_walk[warp - 2];
+                TcPiece to;
+                bool found = false;
+                while (!found && at.next(p, to)) found = to.pair * 2 + x < p.items;
+                if (!found) to.b = -1;
+                s_piece[warp - 2][turn ^ 1] = to;
+                s_walk[warp - 2] = at;
+            }
+            __syncwarp();
+            return s_piece[warp - 2][turn ^ 1].b >= 0;
         };
+        if (lane == 0) s_walk[warp - 2] = walk;
         bool more = advance();
         if (more) {
-            fetch_queries(next);
+            fetch_queries(s_piece[warp - 2][turn ^ 1]);
             queries_there();
         }
         while (ok && more) {
-            c = next;
+            turn ^= 1;
+            const volatile TcPiece& c = s_piece[warp - 2][turn];
             const int item = c.pair * 2 + x, h = item / p.tiles, r = (item - h * p.tiles) * TC_ROWS + row;
             const bool real = r < p.a.rows;
             const int t = real ? r % p.a.T : 0;
@@ -440,7 +472,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 tc_fence_after();
                 if (k + 1 == c.k1) {                               // the last product with these queries is done
                     more = advance();
-                    if (more) fetch_queries(next);
+                    if (more) fetch_queries(s_piece[warp - 2][turn ^ 1]);
                 }
                 const int n0 = k * TC_KEYS;
                 const bool tail = n0 + TC_KEYS > c.len;            // new tokens or slots past the end: what is not seen counts as -infinity
@@ -454,6 +486,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
 #pragma unroll
                 for (int i = 0; i < 4; ++i) tmem_ld_32x32b_x32(t_s + i * 32, s[i]);
                 tmem_ld_wait();
+                tc_fence_before();
+                mbar_arrive(&bar.s_read[x]);
                 if (tail) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
@@ -466,12 +500,16 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 for (int e = 0; e < 32; e += 2)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) top[i] = fmaxf(top[i], fmaxf(__int_as_float(s[i][e]), __int_as_float(s[i][e + 1])));
+                if (k > c.k0) {                                    // the weights before these have been multiplied
+                    if (!wait_or_abort_warp(&bar.pv_done[x], n_pv++ & 1, s_abort)) { ok = false; break; }
+                    tc_fence_after();
+                }
                 const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale2;
                 if (__any_sync(0xffffffffu, high > m + TC_LAZY)) {
                     const float m_new = fmaxf(m, high), alpha = m_new == -INFINITY ? 1.0f : exp2_fast(m - m_new);
                     m = m_new;
                     l *= alpha;
-                    if (k > c.k0) {                                // every product into the output so far is done: s_full says so
+                    if (k > c.k0) {
 #pragma unroll 1
                         for (int i = 0; i < D; i += 16) {
                             int o[16];
@@ -485,22 +523,24 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     }
                 }
                 const float ref = m == -INFINITY ? 0.0f : m;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                float2 sum[4] = {};
+                const float2 scale = make_float2(p.scale2, p.scale2), minus = make_float2(-ref, -ref);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     uint32_t w[16];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        const float a = exp2_fast(fmaf(__int_as_float(s[i][2 * e]), p.scale2, -ref));
-                        const float b = exp2_fast(fmaf(__int_as_float(s[i][2 * e + 1]), p.scale2, -ref));
-                        sum[e & 3] += a + b;
-                        w[e] = pack2<T>(a, b);
+                        float2 y = fma_f32x2(make_float2(__int_as_float(s[i][2 * e]), __int_as_float(s[i][2 * e + 1])), scale, minus);
+                        y.x = exp2_fast(y.x);
+                        y.y = exp2_fast(y.y);
+                        sum[e & 3] = add_f32x2(sum[e & 3], y);
+                        w[e] = pack2<T>(y.x, y.y);
                     }
-                    tmem_st_32x32b_x16(t_s + i * 16, w);
+                    tmem_st_32x32b_x16(t_p + i * 16, w);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                l += ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) + ((sum[2].x + sum[2].y) + (sum[3].x + sum[3].y));
                 if (tail && (c.own || x == 0)) {                   // the values of this block, before anything is multiplied by them
-                    const uint32_t tile = c.value_tile(x, k), slot = tile % TC_SLOTS;
+                    const uint32_t tile = c.first + tc_value_tile(c.own, c.k1 - c.k0, k - c.k0, x), slot = tile % TC_SLOTS;
                     if (!wait_or_abort_warp(&bar.full[slot], (tile / TC_SLOTS) & 1, s_abort)) { ok = false; break; }
                     bool bad = false;
                     for (int i = max(0, c.len - n0) * (D / 8) + row; i < TC_KEYS * (D / 8); i += TC_ROWS) {
@@ -517,15 +557,18 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     if (bad) *reinterpret_cast<volatile int*>(&s_odd) = 1;
                     fence_proxy_async_smem();
                     __syncwarp();
+                    if (c.streams == 2 && !c.own) mbar_arrive(&bar.v_checked);
+                } else if (tail) {
+                    if (!wait_or_abort_warp(&bar.v_checked, n_checked++ & 1, s_abort)) { ok = false; break; }
                 }
                 tmem_st_wait();
                 tc_fence_before();
                 mbar_arrive(&bar.p_full[x]);
             }
             if (ok && more) queries_there();
-            if (!ok || !wait_or_abort_warp(&bar.o_full[x], n_o++ & 1, s_abort)) { ok = false; break; }
+            if (!ok || !wait_or_abort_warp(&bar.pv_done[x], n_pv++ & 1, s_abort)) { ok = false; break; }
             tc_fence_after();
-            const bool whole = c.whole(), odd = *reinterpret_cast<volatile int*>(&s_odd) != 0;
+            const bool whole = c.k0 == 0 && c.k1 == c.blocks, odd = *reinterpret_cast<volatile int*>(&s_odd) != 0;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             const int64_t place = (static_cast<int64_t>(blockIdx.x) * 2 + (c.k0 > 0 ? 0 : 1)) * 2 + x;
             const long long out_row = real ? static_cast<long long>(attn_out_row<T>(p.a, c.b, h, r) - static_cast<T*>(p.a.out)) : -1;
@@ -573,8 +616,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     for (int e = 0; e < 32; ++e) to[e * TC_ROWS] = f[e];
                 }
             }
-            tc_fence_before();
-            mbar_arrive(&bar.o_free[x]);
+            tc_fence_before();                                     // before the next piece's weights, which say that the output may be overwritten
         }
     }
     tc_fence_before();
