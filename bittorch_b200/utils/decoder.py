@@ -25,13 +25,19 @@ Two ways to run a single-token step: ``forward(tokens, cache, pos0)`` with the p
 every shape fixed (attention runs over the whole cache under a mask), which is what a CUDA graph can replay:
 ``GreedyDecodeGraph`` captures one such step, the arg-max and the position increment, so that a decoded token
 costs one graph launch and no host synchronisation.
+
+Serving on top of that uses the operators over the key/value cache (``bittorch_b200.ops``: ``tree_attention``,
+``evict_cache``, ``beam_select``, ``reorder_cache``; CUDA only): ``decode_tokens`` runs any number of new tokens per
+sequence against caches of different lengths, ``decode_tree`` / ``accept_tree`` / ``generate_speculative`` verify trees of
+drafted tokens, ``generate_beam`` searches with beams, ``generate_evicting`` decodes within a bounded cache.  With
+``DecoderConfig.fused_attention`` the single-token step uses ``tree_attention`` too.
 """
 
 from __future__ import annotations
 
 import math
 from dataclasses import dataclass
-from typing import List, Optional, Tuple
+from typing import Callable, List, Optional, Tuple
 
 import torch
 import torch.nn as nn
@@ -57,6 +63,7 @@ class DecoderConfig:
     backend: str = "auto"
     one_weight_copy: bool = True              # inference form: keep only the tiled copy of every projection on the device
     fused_elementwise: bool = True            # inference form, integer path: residual add + RMSNorm and SiLU * up run inside the quantizer kernels
+    fused_attention: bool = False             # fixed-shape step, outside autograd: attention as one operator (ops.tree_attention) that reads the filled slots only
 
     def __post_init__(self) -> None:
         if self.n_kv_heads is None:
@@ -107,6 +114,25 @@ def apply_rope_at(x: Tensor, cos: Tensor, sin: Tensor, pos: Tensor) -> Tensor:
     s = sin.index_select(0, pos)[None, None].to(x.dtype)
     x0, x1 = x[..., :half], x[..., half:]
     return torch.cat([x0 * c - x1 * s, x0 * s + x1 * c], dim=-1)
+
+
+def apply_rope_positions(x: Tensor, cos: Tensor, sin: Tensor, positions: Tensor) -> Tensor:
+    """x: [B, H, T, head_dim]; as ``apply_rope`` with a position per token, positions [B, T]."""
+    half = x.shape[3] // 2
+    c = cos[positions][:, None].to(x.dtype)                          # [B, 1, T, half]
+    s = sin[positions][:, None].to(x.dtype)
+    x0, x1 = x[..., :half], x[..., half:]
+    return torch.cat([x0 * c - x1 * s, x0 * s + x1 * c], dim=-1)
+
+
+@dataclass
+class CacheStep:
+    """Where the new tokens of a step go: token t of sequence b into slot ``lengths[b] + t`` of the cache, rotated by
+    ``positions[b, t]``, seeing the filled slots and, among the new tokens, what ``tree`` says (None: causal)."""
+
+    lengths: Tensor                           # int64 [B]
+    positions: Tensor                         # int64 [B, T]
+    tree: Optional[Tensor] = None             # bool [T, T] or [B, T, T]
 
 
 def fuse_inference_columns(layers, share: bool = False) -> TernaryLinearInference:
@@ -256,6 +282,11 @@ class Attention(nn.Module):
         k_cache, v_cache = cache
         k_cache.index_copy_(2, pos, apply_rope_at(k, cos, sin, pos).to(k_cache.dtype))
         v_cache.index_copy_(2, pos, v.to(v_cache.dtype))
+        if cfg.fused_attention and not (torch.is_grad_enabled() and q.requires_grad):
+            from ..ops import tree_attention
+
+            out = tree_attention(q.to(k_cache.dtype), k_cache, v_cache, pos)
+            return out.transpose(1, 2).reshape(b, 1, cfg.dim).to(q.dtype)
         seq = k_cache.shape[2]
         qg = q.reshape(b, nkv, nh // nkv, hd)                                    # query head h = kv head * group + g
         scores = torch.matmul(qg, k_cache.to(q.dtype).transpose(2, 3)) * (1.0 / math.sqrt(hd))     # [B, Hkv, group, S]
@@ -264,9 +295,37 @@ class Attention(nn.Module):
         out = torch.matmul(torch.softmax(scores, dim=-1).to(q.dtype), v_cache.to(q.dtype))          # [B, Hkv, group, hd]
         return out.reshape(b, 1, cfg.dim)
 
+    def _attend_slots(self, q: Tensor, k: Tensor, v: Tensor, cache, step: CacheStep, cos: Tensor, sin: Tensor) -> Tensor:
+        """The same for T tokens per sequence at the slots and positions of ``step`` -> [B, T, dim].  ``cache`` is (keys,
+        values), or (keys, values, mass) whose third part collects every slot's attention weight."""
+        from ..ops import tree_attention
+
+        b, _, t, _ = q.shape
+        k_cache, v_cache = cache[:2]
+        row = torch.arange(b, device=q.device)[:, None]
+        slot = step.lengths[:, None] + torch.arange(t, device=q.device)          # [B, T]
+        q = apply_rope_positions(q, cos, sin, step.positions)
+        k = apply_rope_positions(k, cos, sin, step.positions)
+        k_cache.transpose(1, 2).index_put_((row, slot), k.transpose(1, 2).to(k_cache.dtype))
+        v_cache.transpose(1, 2).index_put_((row, slot), v.transpose(1, 2).to(v_cache.dtype))
+        out = tree_attention(q.to(k_cache.dtype), k_cache, v_cache, step.lengths, step.tree, mass=cache[2] if len(cache) > 2 else None)
+        return out.transpose(1, 2).reshape(b, t, self.cfg.dim).to(q.dtype)
+
+    def attend(self, q: Tensor, k: Tensor, v: Tensor, cache, pos, cos: Tensor, sin: Tensor, fixed: bool) -> Tensor:
+        """Cache update and attention: ``pos`` an integer (T tokens from there on), a device tensor (``fixed``) or a
+        ``CacheStep``."""
+        if isinstance(pos, CacheStep):
+            return self._attend_slots(q, k, v, cache, pos, cos, sin)
+        return self._attend_fixed(q, k, v, cache, pos, cos, sin) if fixed else self._attend(q, k, v, cache, pos, cos, sin)
+
     def forward(self, x: Tensor, cache: Tuple[Tensor, Tensor], pos0: int, cos: Tensor, sin: Tensor) -> Tensor:
         q, k, v = self._qkv(x)
         return self.proj(self._attend(q, k, v, cache, pos0, cos, sin))
+
+    def decode_tokens(self, x: Tensor, cache, step: CacheStep, cos: Tensor, sin: Tensor) -> Tensor:
+        """T tokens per sequence (x [B, T, dim]) at the slots of ``step``."""
+        q, k, v = self._qkv(x)
+        return self.proj(self._attend_slots(q, k, v, cache, step, cos, sin))
 
     def decode_step(self, x: Tensor, cache: Tuple[Tensor, Tensor], pos: Tensor, cos: Tensor, sin: Tensor) -> Tensor:
         """One token per sequence (x [B, 1, dim]) at the position in the device tensor ``pos``: fixed shapes."""
@@ -314,6 +373,10 @@ class Block(nn.Module):
         x = x + self.attn.decode_step(self.norm1(x), cache, pos, cos, sin)
         return x + self.mlp(self.norm2(x))
 
+    def decode_tokens(self, x: Tensor, cache, step: CacheStep, cos: Tensor, sin: Tensor) -> Tensor:
+        x = x + self.attn.decode_tokens(self.norm1(x), cache, step, cos, sin)
+        return x + self.mlp(self.norm2(x))
+
     def fused_elementwise_ok(self) -> bool:
         """The block can run with its elementwise steps inside the quantizer kernels: every projection packed, the
         integer activation path selected."""
@@ -332,7 +395,8 @@ class Block(nn.Module):
 
         ``x`` [B, T, dim] is the residual stream, updated IN PLACE; ``delta`` is what the previous block's MLP still
         owes it (None for the first block).  Returns (x, d): the caller (next block, or the final norm) adds d.
-        ``fixed``: one token at the position in the device tensor ``pos``; else T tokens from the integer ``pos``."""
+        ``fixed``: one token at the position in the device tensor ``pos``; else T tokens from the integer ``pos``, or at the
+        slots of the ``CacheStep`` ``pos``."""
         from .._ext import require_ext
 
         C = require_ext()
@@ -342,7 +406,7 @@ class Block(nn.Module):
         attn = self.attn
         qkv = attn.fused_columns().fused().forward_quantized(xq, sx, xsum, x.dtype)
         q, k, v = attn._heads(qkv[:, :attn.q_proj.out_features], qkv[:, attn.q_proj.out_features:], b, t)
-        out = attn._attend_fixed(q, k, v, cache, pos, cos, sin) if fixed else attn._attend(q, k, v, cache, pos, cos, sin)
+        out = attn.attend(q, k, v, cache, pos, cos, sin, fixed)
         a = attn.proj(out)
         xq, sx, xsum = C.add_rmsnorm_quant(x2d, a.reshape(b * t, d), self.norm2.weight, NORM_EPS)
         gate_up = self.mlp.fused_columns().fused().forward_quantized(xq, sx, xsum, x.dtype)     # [M, gate | up]
@@ -424,6 +488,175 @@ class TernaryDecoder(nn.Module):
             if i + 1 < new_tokens:
                 nxt = self.forward(nxt, cache, t + i)[:, -1].argmax(dim=-1, keepdim=True)
         return torch.cat(out, dim=1)
+
+    # ---- serving: trees of drafted tokens, beams, bounded caches (operators over the cache; CUDA only) ----------------
+
+    def decode_tokens(self, tokens: Tensor, cache: list, step: CacheStep) -> Tensor:
+        """tokens [B, T] at the slots and positions of ``step`` -> logits [B, T, vocab].  Writes the tokens' keys and values
+        to slots ``step.lengths[b] + t``, which the caller keeps inside the cache, and leaves ``step.lengths`` alone."""
+        x = self.tok(tokens)
+        if self._fused_blocks():
+            return self._run_fused(x, cache, step, fixed=False)
+        for block, layer_cache in zip(self.blocks, cache):
+            x = block.decode_tokens(x, layer_cache, step, self.rope_cos, self.rope_sin)
+        return self.head(self.norm(x))
+
+    def _room(self, cache: list, lengths: Tensor, tokens: int) -> None:
+        """Refuses a step that would write past the cache (reads ``lengths`` back, except while a graph is captured)."""
+        slots = cache[0][0].shape[2] if cache else self.cfg.max_seq_len
+        if tokens > slots or (not torch.cuda.is_current_stream_capturing() and int(lengths.max()) + tokens > slots):
+            raise ValueError(f"{tokens} new tokens do not fit behind the filled part of a cache of {slots} slots")
+
+    @torch.no_grad()
+    def decode_tree(self, tokens: Tensor, cache: list, lengths: Tensor, tree: Tensor) -> Tensor:
+        """Logits [B, T, vocab] of the T drafted tokens [B, T] of a token tree per sequence, in one pass: ``tree`` is
+        ``ops.tree_mask(parents)``, bool [T, T] or [B, T, T].  Node t goes to slot ``lengths[b] + t`` and takes the position
+        of its depth in the tree behind the ``lengths[b]`` committed tokens.  ``accept_tree`` says which nodes stay."""
+        self._room(cache, lengths, tokens.shape[1])
+        depth = (tree.sum(dim=-1) - 1).clamp(min=0)                              # [T] or [B, T]
+        positions = (lengths[:, None] + depth).clamp(max=self.cfg.max_seq_len - 1)
+        return self.decode_tokens(tokens, cache, CacheStep(lengths, positions, tree))
+
+    @torch.no_grad()
+    def accept_tree(self, tokens: Tensor, parents: Tensor, tree: Tensor, logits: Tensor, cache: list, lengths: Tensor):
+        """Greedy verification of a drafted tree whose node 0 is the root (the token that was already chosen): a node stays
+        if its parent stays and its token is the arg-max of its parent's logits.  The longest such path is moved together
+        in the cache (``ops.compact_cache``) -> (path [B, T]: the nodes that stay, in order, then -1; counts [B]; the token
+        that follows the path [B, 1]).  The new lengths are ``lengths + counts``."""
+        from ..ops import compact_cache
+
+        b, t = tokens.shape
+        node = torch.arange(t, device=tokens.device)
+        parents, tree = parents.expand(b, t), tree.expand(b, t, t)
+        choice = logits.argmax(dim=-1)                                           # [B, T]
+        fits = (tokens == choice.gather(1, parents.clamp(min=0).long())) & (parents >= 0)
+        fits[:, 0] = True
+        stays = tree[:, node, node] & ~(tree & ~fits[:, None]).any(dim=-1)       # every ancestor fits, and so does the node
+        depth = torch.where(stays, tree.sum(dim=-1), 0)
+        last = depth.argmax(dim=-1)                                              # the deepest; the root if nothing fits
+        on_path = tree[torch.arange(b, device=tokens.device), last]              # [B, T]
+        counts = on_path.sum(dim=-1)
+        path = torch.where(on_path, node, t).sort(dim=-1).values
+        keep = (lengths[:, None] + path)[:, None]                                # [B, 1, T]; the entries past counts are not used
+        for layer_cache in cache:
+            compact_cache(layer_cache[0], layer_cache[1], keep, counts, lengths)
+        return torch.where(path < t, path, -1), counts, choice.gather(1, last[:, None])
+
+    @torch.no_grad()
+    def generate_speculative(self, prompt: Tensor, new_tokens: int, draft: Callable[[Tensor, Tensor], Tuple[Tensor, Tensor]]) -> Tensor:
+        """Greedy decoding that verifies drafted trees: the tokens of ``generate_greedy``, several per pass where the draft
+        is right.  ``draft(sequence [B, n] padded with -1, current [B, 1])`` -> (tokens [B, T] with ``current`` as node 0,
+        parents int64 [T] or [B, T], ``parents[0] = -1``).  -> [B, prompt + new_tokens]."""
+        from ..ops import tree_mask
+
+        b, t0 = prompt.shape
+        total = t0 + new_tokens
+        if total > self.cfg.max_seq_len:
+            raise ValueError(f"positions up to {total} exceed max_seq_len={self.cfg.max_seq_len}")
+        cache = self.new_cache(b)
+        current = self.forward(prompt, cache, 0, last_only=True)[:, -1].argmax(dim=-1, keepdim=True)
+        lengths = torch.full((b,), t0, dtype=torch.int64, device=prompt.device)
+        out = torch.full((b, self.cfg.max_seq_len + 1), -1, dtype=torch.long, device=prompt.device)
+        out[:, :t0] = prompt
+        row = torch.arange(b, device=prompt.device)[:, None]
+        while int(lengths.min()) < total:
+            at = lengths.clamp(max=total - 1)                                    # a finished sequence runs along on its last token
+            tokens, parents = draft(out[:, :int(lengths.max())], current)
+            t = min(tokens.shape[1], self.cfg.max_seq_len - int(at.max()))
+            tokens, parents = tokens[:, :t], parents[..., :t]
+            tree = tree_mask(parents)
+            logits = self.decode_tree(tokens, cache, at, tree)
+            path, counts, follows = self.accept_tree(tokens, parents, tree, logits, cache, at)
+            slot = lengths[:, None] + torch.arange(t, device=prompt.device)
+            slot = torch.where((path >= 0) & (slot < total), slot, self.cfg.max_seq_len)      # the last column is thrown away
+            out[row, slot] = tokens.gather(1, path.clamp(min=0))
+            current = torch.where(lengths[:, None] < total, follows, current)
+            lengths = (lengths + counts).clamp(max=total)
+        return out[:, :total]
+
+    @torch.no_grad()
+    def generate_beam(self, prompt: Tensor, beams: int, new_tokens: int, end_token: Optional[int] = None) -> Tuple[Tensor, Tensor]:
+        """Beam search: prompt [B, T] -> (sequences [B, beams, T + new_tokens], best first, and their log-probabilities
+        float32 [B, beams]).  A beam that has produced ``end_token`` keeps its score and repeats that token."""
+        from ..ops import beam_select, reorder_cache
+
+        b, t = prompt.shape
+        if t + new_tokens > self.cfg.max_seq_len:
+            raise ValueError(f"positions up to {t + new_tokens} exceed max_seq_len={self.cfg.max_seq_len}")
+        if new_tokens < 1:
+            raise ValueError("beam search needs at least one new token")
+        dev = prompt.device
+        first = self.new_cache(b)
+        logits = self.forward(prompt, first, 0, last_only=True)
+        cache = self.new_cache(b * beams)
+        for (k0, v0), (k, v) in zip(first, cache):
+            for src, dst in ((k0, k), (v0, v)):
+                dst[:, :, :t] = src[:, :, :t].repeat_interleave(beams, dim=0)
+        del first
+        tensors = [x for layer in cache for x in layer]
+        scores, tokens, _ = beam_select(logits, torch.zeros((b, 1), device=dev), beams)
+        history = torch.empty((b, beams, t + new_tokens), dtype=torch.long, device=dev)
+        history[:, :, :t] = prompt[:, None]
+        history[:, :, t] = tokens
+        finished = None if end_token is None else tokens == end_token
+        pos = torch.full((1,), t, dtype=torch.long, device=dev)
+        for i in range(1, new_tokens):
+            logits = self.decode_step(tokens.reshape(b * beams, 1), cache, pos)
+            scores, tokens, parents = beam_select(logits.reshape(b, beams, -1), scores, beams, finished, end_token)
+            pos = pos + 1
+            reorder_cache(tensors, parents, pos, start=t)
+            history[:, :, t:t + i] = history[:, :, t:t + i].gather(1, parents[..., None].expand(b, beams, i))
+            history[:, :, t + i] = tokens
+            if finished is not None:
+                finished = finished.gather(1, parents) | (tokens == end_token)
+        return history, scores
+
+    @torch.no_grad()
+    def generate_evicting(self, prompt: Tensor, new_tokens: int, budget: int, sinks: int = 4, recent: Optional[int] = None,
+                          window: int = 32, slack: int = 64) -> Tensor:
+        """Greedy decoding within a cache of ``budget + slack`` slots per sequence and head: prompt [B, T] -> [B, T +
+        new_tokens].  The last ``window`` prompt tokens and every decoded one add their attention weights up per slot; when
+        the cache is full, the first ``sinks`` and the last ``recent`` (default: half the budget) slots stay, and the
+        heaviest of the others (``ops.evict_cache``).  Keys keep the rotation of their own positions."""
+        from ..ops import evict_cache
+
+        b, t = prompt.shape
+        if t + new_tokens > self.cfg.max_seq_len:
+            raise ValueError(f"positions up to {t + new_tokens} exceed max_seq_len={self.cfg.max_seq_len}")
+        recent = (budget - sinks) // 2 if recent is None else recent
+        if slack < 1:
+            raise ValueError("slack must be at least one slot")
+        dev = prompt.device
+        full = self.new_cache(b)
+        mass = lambda k: torch.zeros(k.shape[:3], dtype=torch.float32, device=dev)
+        full = [(k, v, mass(k)) for k, v in full]
+        head = t - min(window, t)
+        if head > 0:
+            self.forward(prompt[:, :head], [c[:2] for c in full], 0, last_only=True)
+        lengths = torch.full((b,), head, dtype=torch.int64, device=dev)
+        positions = torch.arange(head, t, device=dev).expand(b, t - head)
+        current = self.decode_tokens(prompt[:, head:], full, CacheStep(lengths, positions))[:, -1].argmax(dim=-1, keepdim=True)
+        lengths = torch.full((b,), t, dtype=torch.int64, device=dev)
+        out = [prompt, current]
+        cfg = self.cfg
+        cache = []
+        for k, v, m in full:                                                     # into caches of the bounded size
+            small = tuple(torch.zeros((b, cfg.n_kv_heads, budget + slack, cfg.head_dim), dtype=k.dtype, device=dev) for _ in range(2))
+            small += (torch.zeros((b, cfg.n_kv_heads, budget + slack), dtype=torch.float32, device=dev),)
+            _, counts = evict_cache(k, v, m, lengths, budget, sinks, recent, out=small)
+            cache.append(small)
+        del full
+        lengths, filled = counts, min(t, budget)
+        for i in range(1, new_tokens):
+            if filled == budget + slack:
+                for k, v, m in cache:
+                    _, counts = evict_cache(k, v, m, lengths, budget, sinks, recent)
+                lengths, filled = counts, budget
+            positions = torch.full((b, 1), t + i - 1, dtype=torch.long, device=dev)
+            current = self.decode_tokens(current, cache, CacheStep(lengths, positions))[:, -1].argmax(dim=-1, keepdim=True)
+            out.append(current)
+            lengths, filled = lengths + 1, filled + 1
+        return torch.cat(out[:1 + new_tokens], dim=1)
 
     def to_inference(self) -> "TernaryDecoder":
         """Replaces every ternary projection by its packed inference form (2-bit weights, fused kernels); the
