@@ -299,6 +299,44 @@ def compact_cache(k: Tensor, v: Tensor, keep: Tensor, counts: Tensor, first: Opt
 
 
 @functools.lru_cache(maxsize=1024)
+def _evict_cache_plan(k_sig, v_sig, mass_sig, len_sig, budget, sinks, recent, out_sigs):
+    if len(k_sig[0]) != 4 or mass_sig[0] != k_sig[0][:3]:
+        _fail(f"mass must be float32 {list(k_sig[0][:3])}, got {mass_sig[2]} {list(mass_sig[0])}")
+    if out_sigs is not None and (len(out_sigs) != 3 or len(out_sigs[0][0]) != 4 or out_sigs[0][0][2] < budget):
+        _fail(f"out must be (keys, values, mass) of at least {budget} slots")
+    b, hkv = mass_sig[0][:2]
+    select = _evict_plan(mass_sig, len_sig, budget, sinks, recent)
+    keep = (torch.Size((b, hkv, budget)), (hkv * budget, budget, 1), torch.int64)
+    return select, _compact_plan(k_sig, v_sig, keep, (torch.Size((b,)), (1,), torch.int64), None, mass_sig, out_sigs)
+
+
+def evict_cache(k: Tensor, v: Tensor, mass: Tensor, lengths: Tensor, budget: int, sinks: int, recent: int,
+                out: Optional[Sequence[Tensor]]) -> Tuple[Tensor, Tensor]:
+    budget, sinks, recent = int(budget), int(sinks), int(recent)
+    (sizes, strides, lens), (head, tail, mass_strides) = _evict_cache_plan(
+        _sig(k), _sig(v), _sig(mass), _sig(lengths), budget, sinks, recent, None if out is None else tuple([_sig(x) for x in out]))
+    k_out, v_out, mass_out = (k, v, mass) if out is None else out
+    if torch.is_grad_enabled():
+        _no_gradient("evict_cache", k, v, k_out, v_out, mass, mass_out)
+    k_at, v_at, mass_at = k.data_ptr(), v.data_ptr(), mass.data_ptr()
+    if out is None:
+        k_to, v_to, mass_to = k_at, v_at, mass_at
+        index = _same_device("evict_cache", k, v, mass, lengths)
+    else:
+        k_to, v_to, mass_to = k_out.data_ptr(), v_out.data_ptr(), mass_out.data_ptr()
+        if k_to in (k_at, v_at) or v_to in (k_at, v_at, k_to) or mass_to == mass_at:
+            _fail("out must be other memory than the cache (leave it out to evict in place)")
+        index = _same_device("evict_cache", k, v, mass, lengths, k_out, v_out, mass_out)
+    b, hkv, _ = sizes
+    keep = torch.empty((b, hkv, budget), dtype=torch.int64, device=k.device)
+    counts = torch.empty((b,), dtype=torch.int64, device=k.device)
+    keep_at, counts_at = keep.data_ptr(), counts.data_ptr()
+    _call(index, _evict_select, mass_at, *strides, *sizes, lengths.data_ptr(), *lens, budget, sinks, recent, keep_at, counts_at)
+    _call(index, _compact_cache, k_at, v_at, k_to, v_to, *head, keep_at, *tail, counts_at, None, mass_at, mass_to, mass_strides)
+    return keep, counts
+
+
+@functools.lru_cache(maxsize=1024)
 def _beam_plan(logits_sig, scores_sig, select, finished_sig, end_token):
     logits, scores, finished = (None if x is None else torch.empty_strided(x[0], x[1], dtype=x[2], device="meta")
                                 for x in (logits_sig, scores_sig, finished_sig))

@@ -340,8 +340,9 @@ struct Candidate {
     }
 };
 
-// Entry e of the list that piece `piece` of beam w left
-__device__ __forceinline__ Candidate beam_candidate(const BeamParams& p, int64_t b, int w, int piece, int e, const double* s_base,
+// Entry e of the list that piece `piece` of beam w left.  (One copy of the code: what a kernel this short spends most of its
+// time on is fetching its instructions.)
+__device__ __noinline__ Candidate beam_candidate(const BeamParams& p, int64_t b, int w, int piece, int e, const double* s_base,
                                                     const uint8_t* s_kind) {
     Candidate c = {-INFINITY, -1};
     int64_t token;
@@ -365,7 +366,7 @@ __device__ __forceinline__ Candidate beam_candidate(const BeamParams& p, int64_t
 
 constexpr int BJ_THREADS = 256;
 
-__global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const BeamParams p) {
+__global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const __grid_constant__ BeamParams p) {
     __shared__ double s_base[BT_BEAM_MAX_BEAMS];                   // score - log-sum
     __shared__ uint8_t s_kind[BT_BEAM_MAX_BEAMS];                  // 0 live, 1 finished, 2 nothing but -infinity
     __shared__ Candidate s_best[BJ_THREADS];
@@ -420,8 +421,7 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const BeamParams 
     }
     __syncthreads();
     const Candidate edge = s_edge;
-#pragma unroll 4
-    for (unsigned i = tid; i < lists * p.n; i += BJ_THREADS) {     // all entries: their loads do not wait for one another
+    for (unsigned i = tid; i < lists * p.n; i += BJ_THREADS) {
         const unsigned list = i / p.n, w = list / p.pieces;
         const Candidate c = beam_candidate(p, b, w, list - w * p.pieces, i - list * p.n, s_base, s_kind);
         if (c.place < 0 || edge.better(c)) continue;

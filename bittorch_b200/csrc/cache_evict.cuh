@@ -18,7 +18,6 @@
 
 namespace bt {
 
-constexpr int EV_THREADS = 1024;
 
 struct EvictParams {
     const float* mass;
@@ -38,7 +37,7 @@ __device__ __forceinline__ uint32_t ordered_key(float x) {
 }
 
 // IPT: neighbouring slots of a thread.
-template <int IPT>
+template <int EV_THREADS, int IPT>
 __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictParams p) {
     constexpr int BLOCK = EV_THREADS * IPT;
     __shared__ int s_hist[256 * 32];                               // [digit][lane]
@@ -88,17 +87,16 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictPar
     uint32_t prefix = 0;                                           // the digits of the k-th largest key that are known
     int want = static_cast<int>(p.budget) - p.sinks - p.recent;    // it is the want-th largest of those with this prefix
     int shift = 32;                                                // bits not yet known
-#pragma unroll
-    for (int pass = 0; pass < 4; ++pass) {
-        if (want == 0) break;
-        shift = 24 - 8 * pass;
+#pragma unroll 1                                                   // four copies of the code cost more to fetch than they save
+    while (want > 0 && shift > 0) {
+        shift -= 8;
         for (int i = tid; i < 256 * 32; i += EV_THREADS) s_hist[i] = 0;
         __syncthreads();
         for (int blk = 0; blk < blocks; ++blk) {
             if (blocks > 1) competitors(blk * BLOCK + tid * IPT);
 #pragma unroll
             for (int i = 0; i < IPT; ++i)
-                if (pass == 0 || (key[i] >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&s_hist[((key[i] >> shift) & 255u) * 32 + lane], 1);
+                if (((key[i] ^ prefix) >> shift) < 256u) atomicAdd(&s_hist[((key[i] >> shift) & 255u) * 32 + lane], 1);
         }
         __syncthreads();
 #pragma unroll
@@ -159,7 +157,7 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictPar
         }
         if (lane == 31) s_warp[warp] = upto;
         __syncthreads();
-        unsigned all = s_warp[lane];
+        unsigned all = lane < EV_THREADS / 32 ? s_warp[lane] : 0u;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const unsigned x = __shfl_up_sync(0xffffffffu, all, o);
@@ -339,10 +337,12 @@ extern "C" int bt_evict_select(const float* mass, int64_t mass_sb, int64_t mass_
     p.sinks = static_cast<int>(sinks); p.recent = static_cast<int>(recent);
     p.budget = budget; p.keep = keep; p.counts = counts;
     const dim3 grid(static_cast<unsigned>(B * Hkv));
-    // the shortest run of slots per thread that holds the cache in registers; a longer cache is read again in every pass
-    if (S <= 4 * EV_THREADS) return launch_early(evict_select_kernel<4>, "evict_select_kernel", grid, EV_THREADS, 0, stream, p);
-    if (S <= 16 * EV_THREADS) return launch_early(evict_select_kernel<16>, "evict_select_kernel", grid, EV_THREADS, 0, stream, p);
-    return launch_early(evict_select_kernel<32>, "evict_select_kernel", grid, EV_THREADS, 0, stream, p);
+    // The shortest run of slots per thread that holds the cache in registers; a longer cache is read again in every pass.
+    // Short caches: a CTA of 1024 threads is the fastest for one head, many heads go faster through CTAs of 256.
+    if (S <= 4096 && grid.x <= static_cast<unsigned>(sm_count())) return launch_early(evict_select_kernel<1024, 4>, "evict_select_kernel", grid, 1024, 0, stream, p);
+    if (S <= 4096) return launch_early(evict_select_kernel<256, 16>, "evict_select_kernel", grid, 256, 0, stream, p);
+    if (S <= 16384) return launch_early(evict_select_kernel<1024, 16>, "evict_select_kernel", grid, 1024, 0, stream, p);
+    return launch_early(evict_select_kernel<1024, 32>, "evict_select_kernel", grid, 1024, 0, stream, p);
 }
 
 extern "C" int bt_compact_cache(const void* k, const void* v, void* k_out, void* v_out, int dtype, int64_t B, int64_t Hkv,

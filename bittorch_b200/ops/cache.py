@@ -92,14 +92,7 @@ def evict_cache(k_cache: Tensor, v_cache: Tensor, mass: Tensor, lengths: Tensor,
                 recent: int = 0, out: Optional[Sequence[Tensor]] = None) -> Tuple[Tensor, Tensor]:
     """Cuts a cache down to ``budget`` slots per sequence and head: ``evict_select``, then ``compact_cache`` of keys, values
     and mass, in place or into ``out`` = (keys, values, mass) with at least ``budget`` slots.  -> (keep, counts)."""
-    binding = _binding()
-    if k_cache.dim() != 4 or mass.shape != k_cache.shape[:3]:
-        raise RuntimeError(f"mass must be float32 {list(k_cache.shape[:3])}, got {mass.dtype} {list(mass.shape)}")
-    if out is not None and (len(out) != 3 or out[0].dim() != 4 or out[0].shape[2] < budget):
-        raise RuntimeError(f"out must be (keys, values, mass) of at least {budget} slots")
-    keep, counts = binding.evict_select(mass, lengths, budget, sinks, recent)
-    binding.compact_cache(k_cache, v_cache, keep, counts, None, mass, out)
-    return keep, counts
+    return _binding().evict_cache(k_cache, v_cache, mass, lengths, budget, sinks, recent, out)
 
 
 def beam_select(logits: Tensor, scores: Tensor, select: Optional[int] = None, finished: Optional[Tensor] = None,
