@@ -40,7 +40,7 @@ __device__ __forceinline__ uint32_t ordered_key(float x) {
 template <int EV_THREADS, int IPT>
 __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictParams p) {
     constexpr int BLOCK = EV_THREADS * IPT;
-    __shared__ int s_hist[256 * 32];                               // [digit][lane]
+    __shared__ int s_hist[257 * 32];                               // [digit][lane]; the last row takes the keys with another prefix
     __shared__ int s_digit[256];
     __shared__ unsigned s_warp[EV_THREADS / 32];
     __shared__ uint32_t s_prefix;
@@ -95,8 +95,7 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(const EvictPar
         for (int blk = 0; blk < blocks; ++blk) {
             if (blocks > 1) competitors(blk * BLOCK + tid * IPT);
 #pragma unroll
-            for (int i = 0; i < IPT; ++i)
-                if (((key[i] ^ prefix) >> shift) < 256u) atomicAdd(&s_hist[((key[i] >> shift) & 255u) * 32 + lane], 1);
+            for (int i = 0; i < IPT; ++i) atomicAdd(&s_hist[min((key[i] ^ prefix) >> shift, 256u) * 32 + lane], 1);
         }
         __syncthreads();
 #pragma unroll

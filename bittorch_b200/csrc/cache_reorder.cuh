@@ -23,8 +23,9 @@ struct ReorderParams {
     int blocks;                                                    // CTAs per tensor, group and head
 };
 
+// (Up to eight beams: at least 48 warps an SM, 16 x 4001 slots of 8 beams 361 us instead of 405 us.)
 template <typename U, int WMAX>
-__global__ void __launch_bounds__(RO_THREADS) reorder_cache_kernel(const __grid_constant__ ReorderParams p) {
+__global__ void __launch_bounds__(RO_THREADS, WMAX <= 8 ? 6 : 1) reorder_cache_kernel(const __grid_constant__ ReorderParams p) {
     __shared__ int s_parent[WMAX];
     const int tid = threadIdx.x;
     const int at = static_cast<int>(blockIdx.x / static_cast<unsigned>(p.blocks)), blk = static_cast<int>(blockIdx.x) - at * p.blocks;
