@@ -204,6 +204,9 @@ def tree_attention(q: Tensor, k: Tensor, v: Tensor, lengths: Tensor, tree: Optio
         _no_gradient("tree_attention", q, k, v, mass, out)
     index = _same_device("tree_attention", q, k, v, lengths, tree, mass, out)
     head, lens, tree_sb, mass_strides, need, out_strides = plan
+    if out is not None and out.untyped_storage().data_ptr() in (q.untyped_storage().data_ptr(), k.untyped_storage().data_ptr(),
+                                                                v.untyped_storage().data_ptr()):
+        _fail("out must be other memory than the queries and the cache")
     if q.stride(3) != 1:
         q = q.contiguous()
     if tree is not None and not tree.is_contiguous():
@@ -288,6 +291,8 @@ def compact_cache(k: Tensor, v: Tensor, keep: Tensor, counts: Tensor, first: Opt
         apart = [x.data_ptr() for x in (k, v, k_out, v_out)]
         if apart[2] in apart[:2] or apart[3] in apart[:3] or (mass is not None and mass_out.data_ptr() == mass.data_ptr()):
             _fail("out must be other memory than the cache (leave it out to compact in place)")
+    elif k.data_ptr() == v.data_ptr():
+        _fail("keys and values that are the same memory cannot be compacted in place")
     index = _same_device("compact_cache", k, v, k_out, v_out, keep, counts, first, mass, mass_out)
     if keep.stride(2) != 1:
         keep = keep.contiguous()
@@ -320,6 +325,8 @@ def evict_cache(k: Tensor, v: Tensor, mass: Tensor, lengths: Tensor, budget: int
         _no_gradient("evict_cache", k, v, k_out, v_out, mass, mass_out)
     k_at, v_at, mass_at = k.data_ptr(), v.data_ptr(), mass.data_ptr()
     if out is None:
+        if k_at == v_at:
+            _fail("keys and values that are the same memory cannot be evicted from in place")
         k_to, v_to, mass_to = k_at, v_at, mass_at
         index = _same_device("evict_cache", k, v, mass, lengths)
     else:

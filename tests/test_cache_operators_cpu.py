@@ -114,6 +114,9 @@ def test_the_other_operators_refuse():
     refuses("third", ops.compact_cache, k, k.clone(), keep, n, mass=mass, out=(k.clone(), k.clone()))
     refuses("other memory", ops.compact_cache, k, k.clone(), keep, n, out=(k, k.clone()))
     refuses("share no memory", ops.compact_cache, k[:, :1].expand(2, 3, 10, 8), k.clone(), keep, n)
+    refuses("same memory", ops.compact_cache, k, k, keep, n)
+    refuses("same memory", ops.evict_cache, k, k, mass, n, 4, 1, 1)
+    refuses("other memory", ops.evict_cache, k, k.clone(), mass, n, 4, 1, 1, out=(k, k.clone(), mass.clone()))
     refuses("CUDA", ops.compact_cache, k, k.clone(), keep, n)
     x, s = torch.zeros(2, 3, 50), torch.zeros(2, 3)
     refuses("logits must be", ops.beam_select, x[0], s)

@@ -92,6 +92,31 @@ def test_trees(b, h, hkv, t, s, d, lens, trees, dtype):
     _attention_case(b, h, hkv, t, s, d, lens, dtype, trees, with_mass=t < 20, seed=2, stretch=3.0)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("b,h,hkv,t,s,d,lens,trees", [
+    (2, 9, 3, 16, 700, 128, [0, 650], "each"),               # three heads of one tile each: two together, one alone
+    (2, 8, 2, 75, 400, 64, [320, 129], "one"),               # three tiles a head: two share its keys, the third goes with the next head's
+    (1, 4, 1, 32, 5200, 128, [5100], "one"),                 # fewer blocks than CTAs
+    (9, 4, 2, 20, 1500, 64, [1400, 0, 127, 128, 129, 1, 600, 1280, 256], "each"),
+    (1, 2, 1, 250, 700, 128, [333], "one"), (1, 3, 1, 300, 520, 64, [100], None), (2, 2, 2, 17, 17, 128, [0, 5], None),
+])
+def test_many_rows(b, h, hkv, t, s, d, lens, trees, dtype):
+    """Rows in tiles of 128, pairs of tiles of one head or two, pieces of a sequence on several CTAs."""
+    from bittorch_b200 import _C
+
+    _attention_case(b, h, hkv, t, s, d, lens, dtype, trees, stretch=2.0)
+    assert _C.device_status() == 0
+
+
+@pytest.mark.parametrize("t", [1, 24])
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1.7, 40.0])
+def test_scales(t, scale):
+    """Any finite scale: uniform weights, the smallest products first, weights that are all but one-hot (where a score moves
+    the running maximum by far more than a float's exponent can take)."""
+    for dtype in (torch.float32, torch.bfloat16):
+        _attention_case(2, 4, 2, t, 300, 64, [260, 70], dtype, "one", scale=scale)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("t,d", [(1, 128), (9, 64), (40, 128), (1, 20)])
 def test_other_layouts(t, d, dtype):
@@ -131,6 +156,22 @@ def test_nothing_reaches_a_token_that_does_not_see_it(t, d, g, dtype):
     ops.tree_attention(q, k, v, lengths, blank, mass=mass)
     assert bool((mass[1] == 0).all()) and torch.allclose(mass[0].sum(-1), torch.full((hkv,), float(g * t), device="cuda"), rtol=1e-4)
     assert bool((mass[0, :, n:] == 0).all())
+
+
+def test_values_given_for_the_output_and_expanded_caches():
+    """An output of the caller's with its own strides; a cache that all sequences share (stride 0), read only."""
+    ops = _ops()
+    g = torch.Generator().manual_seed(5)
+    for t, d in ((1, 128), (33, 128), (3, 40)):
+        k, v = (torch.randn(1, 2, 200, d, generator=g).bfloat16().cuda().expand(3, 2, 200, d) for _ in range(2))
+        q = torch.randn(3, 4, t, d, generator=g).bfloat16().cuda()
+        lengths = torch.tensor([150, 0, 199 - t]).cuda()
+        want = ops.tree_attention(q, k.contiguous(), v.contiguous(), lengths)
+        buf = torch.full((3, 4, t, 2 * d), 7.0, dtype=torch.bfloat16, device="cuda")
+        got = ops.tree_attention(q, k, v, lengths, out=buf[..., :d])
+        assert torch.allclose(got.float(), want.float(), rtol=2e-2, atol=2e-2) and bool((buf[..., d:] == 7).all())
+        with pytest.raises(RuntimeError, match="other memory"):
+            ops.tree_attention(q, k, v, lengths, out=q)
 
 
 def test_long_cache_offsets_pass_32_bits():
