@@ -32,6 +32,9 @@ constexpr int TC_SLOTS = 4;                                        // ring of ke
 constexpr int TC_THREADS = 352;                                    // warps: 0 TMA, 1 scores, 10 outputs, 2-5 and 6-9 the streams
 constexpr int TC_COLS = 512;                                       // TMEM: scores at 0, weights at 128 and 192, outputs at 256 and 384
 constexpr int TC_WEIGHTS = 128, TC_OUTPUT = 256;
+// What finishing a pair costs, in blocks: counted when work is dealt out (8 x 61 nodes over up to 8190 slots: 0 138 us, 4 130 us,
+// 8 126 us, 13 129 us).
+constexpr int TC_END = 8;
 constexpr float TC_LAZY = 8.0f;                                    // how far (in powers of 2) a score may exceed the reference point
 
 template <int D> __host__ __device__ constexpr int tc_tile_bytes() { return TC_KEYS * D * 2; }
@@ -59,11 +62,12 @@ struct TcPiece {
 };
 __device__ __forceinline__ int tc_blocks(const AttnTcParams& p, int b) { return (attn_end(p.a, attn_len(p.a, b)) + TC_KEYS - 1) / TC_KEYS; }
 
-// Blocks of the whole line, and where position `pos` lies on it.  Run by whole warps; every lane gets the result.
+// The length of the whole line, in which every pair's blocks are followed by TC_END places without work, and where position
+// `pos` lies on it.  Run by whole warps; every lane gets the result.
 __device__ __forceinline__ int64_t tc_total(const AttnTcParams& p) {
     const int lane = threadIdx.x & 31;
     int64_t sum = 0;
-    for (int b = lane; b < p.a.B; b += 32) sum += tc_blocks(p, b);
+    for (int b = lane; b < p.a.B; b += 32) sum += tc_blocks(p, b) + TC_END;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     return sum * p.pairs;
@@ -73,7 +77,7 @@ __device__ __forceinline__ void tc_locate(const AttnTcParams& p, int64_t pos, in
     int64_t before = 0;
     b = p.a.B, pair = 0, block = 0;
     for (int b0 = 0; b0 < p.a.B; b0 += 32) {
-        const int n = b0 + lane < p.a.B ? tc_blocks(p, b0 + lane) : 0;
+        const int n = b0 + lane < p.a.B ? tc_blocks(p, b0 + lane) + TC_END : 0;
         int64_t upto = static_cast<int64_t>(n) * p.pairs;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -120,18 +124,24 @@ struct TcWalk {
     int64_t left;
     uint32_t tiles;                                                // of keys and values so far
     __device__ __forceinline__ bool next(const AttnTcParams& p, TcPiece& c) {
-        if (left <= 0 || b >= p.a.B) return false;
+        while (true) {
+            if (left <= 0 || b >= p.a.B) return false;
+            c.len = attn_len(p.a, b);
+            c.end = attn_end(p.a, c.len);
+            c.blocks = (c.end + TC_KEYS - 1) / TC_KEYS;
+            if (block < c.blocks) break;
+            left -= c.blocks + TC_END - block;                     // nothing is left of this pair
+            block = 0;
+            if (++pair == p.pairs) pair = 0, ++b;
+        }
         c.b = b; c.pair = pair; c.k0 = block;
-        c.len = attn_len(p.a, b);
-        c.end = attn_end(p.a, c.len);
-        c.blocks = (c.end + TC_KEYS - 1) / TC_KEYS;
         c.k1 = static_cast<int>(c.blocks - block < left ? c.blocks : block + left);
         const int item = pair * 2;
         c.streams = item + 1 < p.items ? 2 : 1;
         c.own = c.streams == 2 && item / p.tiles != (item + 1) / p.tiles;
         c.first = tiles;
         tiles += (c.own ? 4 : 2) * (c.k1 - c.k0);
-        left -= c.k1 - c.k0;
+        left -= c.blocks + TC_END - block;
         block = 0;
         if (++pair == p.pairs) pair = 0, ++b;
         return true;
@@ -470,10 +480,6 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             for (int k = c.k0; k < c.k1; ++k) {
                 if (!wait_or_abort_warp(&bar.s_full[x], n_s++ & 1, s_abort)) { ok = false; break; }
                 tc_fence_after();
-                if (k + 1 == c.k1) {                               // the last product with these queries is done
-                    more = advance();
-                    if (more) fetch_queries(s_piece[warp - 2][turn ^ 1]);
-                }
                 const int n0 = k * TC_KEYS;
                 const bool tail = n0 + TC_KEYS > c.len;            // new tokens or slots past the end: what is not seen counts as -infinity
                 uint32_t sees[4] = {~0u, ~0u, ~0u, ~0u};
@@ -542,16 +548,18 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 if (tail && (c.own || x == 0)) {                   // the values of this block, before anything is multiplied by them
                     const uint32_t tile = c.first + tc_value_tile(c.own, c.k1 - c.k0, k - c.k0, x), slot = tile % TC_SLOTS;
                     if (!wait_or_abort_warp(&bar.full[slot], (tile / TC_SLOTS) & 1, s_abort)) { ok = false; break; }
-                    bool bad = false;
-                    for (int i = max(0, c.len - n0) * (D / 8) + row; i < TC_KEYS * (D / 8); i += TC_ROWS) {
+                    auto at = [&](int i) {                         // 16-byte piece i of the tile's rows
                         const int n = i / (D / 8), chunk = i % (D / 8);
-                        uint4* at = reinterpret_cast<uint4*>(s_kv + slot * TILE + chunk / 8 * BOX + n * 128 + (((chunk & 7) ^ (n & 7)) << 4));
-                        const uint4 v = *at;
-                        if (n0 + n >= c.end) {
-                            *at = make_uint4(0, 0, 0, 0);
-                        } else if (any_nonfinite<T>(v.x) || any_nonfinite<T>(v.y) || any_nonfinite<T>(v.z) || any_nonfinite<T>(v.w)) {
+                        return reinterpret_cast<uint4*>(s_kv + slot * TILE + chunk / 8 * BOX + n * 128 + (((chunk & 7) ^ (n & 7)) << 4));
+                    };
+                    const int from = max(0, c.len - n0), to = min(TC_KEYS, c.end - n0);
+                    bool bad = false;
+                    for (int i = to * (D / 8) + row; i < TC_KEYS * (D / 8); i += TC_ROWS) *at(i) = make_uint4(0, 0, 0, 0);
+                    for (int i = from * (D / 8) + row; i < to * (D / 8); i += TC_ROWS) {
+                        const uint4 v = *at(i);
+                        if (any_nonfinite<T>(v.x) || any_nonfinite<T>(v.y) || any_nonfinite<T>(v.z) || any_nonfinite<T>(v.w)) {
                             bad = true;
-                            *at = make_uint4(finite_only<T>(v.x), finite_only<T>(v.y), finite_only<T>(v.z), finite_only<T>(v.w));
+                            *at(i) = make_uint4(finite_only<T>(v.x), finite_only<T>(v.y), finite_only<T>(v.z), finite_only<T>(v.w));
                         }
                     }
                     if (bad) *reinterpret_cast<volatile int*>(&s_odd) = 1;
@@ -565,7 +573,12 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 tc_fence_before();
                 mbar_arrive(&bar.p_full[x]);
             }
-            if (ok && more) queries_there();
+            if (!ok) break;
+            more = advance();                                      // the last product with these queries is done
+            if (more) {
+                fetch_queries(s_piece[warp - 2][turn ^ 1]);
+                queries_there();
+            }
             if (!ok || !wait_or_abort_warp(&bar.pv_done[x], n_pv++ & 1, s_abort)) { ok = false; break; }
             tc_fence_after();
             const bool whole = c.k0 == 0 && c.k1 == c.blocks, odd = *reinterpret_cast<volatile int*>(&s_odd) != 0;
@@ -643,7 +656,7 @@ __global__ void __launch_bounds__(TC_ROWS) attn_tc_join_kernel(const __grid_cons
     int b, pair, block;
     if (to >= total || to == from) return;
     tc_locate(p, to, b, pair, block);
-    if (block == 0 || to - block < from) return;                   // the cut lies between pairs, or the pair begins in an earlier CTA
+    if (block == 0 || block >= tc_blocks(p, b) || to - block < from) return;       // the cut lies between pairs, or the pair begins in an earlier CTA
     const int64_t end = to - block + tc_blocks(p, b);
     int last = i + 1;                                              // the CTA with the pair's last piece
     while (cuts.at(last + 1) < end) ++last;
