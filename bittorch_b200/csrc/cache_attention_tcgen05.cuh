@@ -5,10 +5,10 @@
 // of one sequence at a time ("streams"): while the tensor cores make one tile's scores, the other tile's threads turn
 // theirs into weights.  Tiles of the same head share the keys and values that TMA brings in; the last tile of a head and
 // the first of the next go together too, each with its own.  A stream's step, for 128 slots:
-//   S = Q K^T   tcgen05.mma, both operands in shared memory, 128 columns of TMEM
+//   S = Q K^T   tcgen05.mma, both operands in shared memory, 128 columns of TMEM that the streams use in turn
 //   weights     a row's 128 scores in its thread's registers; the reference point of the exponentials moves only when a
 //               score exceeds it by 2^8 (the sums stay far from overflow, and the output is almost never rescaled);
-//               the weights, rounded to the cache's type, go back into TMEM where the scores were
+//               the weights, rounded to the cache's type (relative 2^-8 / 2^-11 at most), go to the stream's place in TMEM
 //   O += P V    tcgen05.mma with P from TMEM, V as it lies in the cache (its columns contiguous)
 //
 // Work is dealt out in blocks of 128 slots: the blocks of all pairs of tiles of all sequences form one line, and every
@@ -18,7 +18,12 @@
 //
 // New tokens: scores that a row does not see are masked; values in slots past the end are overwritten with zeros before
 // they are multiplied, and so are infinities and NaN among the new tokens' values, which are added at the end to
-// the rows that see them.  Bound by the tensor cores from about 128 rows on, by HBM below.
+// the rows that see them.
+//
+// 8 trees of 61 nodes over 4099 to 8190 slots, 64 heads over 8, head size 128, fp16: 127 us, 780 TFLOP/s.  A block of two tiles
+// takes about 3350 cycles; its four products need 2048, the 32768 exponentials of the two streams as many (16 a cycle), and
+// the maxima, conversions and TMEM transfers share the issue slots with them: bound by the streams' issue.  Short calls:
+// by 16 to 19 thousand cycles at the end of a pair (output through shared memory, the pieces' join).
 #pragma once
 
 #include "cache_attention_stream.cuh"
@@ -697,9 +702,19 @@ __global__ void __launch_bounds__(TC_ROWS) attn_tc_join_kernel(const __grid_cons
 
 // ---- host side ----------------------------------------------------------------------------------------------------
 
-// Whether a call's sizes are for this kernel (the workspace goes by them); more than one tile of the kernel for few rows.
-static bool attn_tc_sizes(int64_t H, int64_t Hkv, int64_t T, int64_t D, int dtype, bool want_mass) {
-    return dtype != BT_F32 && (D == 64 || D == 128) && !want_mass && H / Hkv * T > AT_ROWS;
+// Whether a call's sizes are for this kernel (the workspace goes by them).  The kernel for few rows takes more rows 16 at a
+// time and reads the cache again for each tile, out of L2; what speaks for it is that a call of it costs 8 us at least,
+// one of this kernel 25 us (tensor memory, barriers, the joining of pieces).  Measured, in us, that kernel / this one
+// (batch x heads / key heads, new tokens, filled slots; head size 128, bf16):
+//   1 x 20/20, 32, 517: 16.7 / 28.0   1 x 64/8, 5, 900: 14.7 / 31.2     1 x 64/8, 5, 16000: 56.6 / 68.0   1 x 32/8, 24, 4000: 41.8 / 54.3
+//   8 x 64/8, 5, 900: 41.0 / 29.5     8 x 32/8, 24, 400: 48.5 / 28.3    1 x 64/8, 61, 400: 32.9 / 29.4    8 x 64/8, 5, 4000: 90.6 / 50.0
+// so the other one where there are few tiles of few rows, or little work in all (the slots are the cache's: how many are
+// filled only the device knows).
+static bool attn_tc_sizes(int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t S, int64_t D, int dtype, bool want_mass) {
+    const int64_t rows = H / Hkv * T, tiles = ceil_div<int64_t>(rows, AT_ROWS), all = B * Hkv * tiles;
+    if (dtype == BT_F32 || (D != 64 && D != 128) || want_mass || tiles == 1) return false;
+    if (rows <= TC_ROWS && all <= 64) return false;
+    return static_cast<double>(all) * static_cast<double>(S) * static_cast<double>(D) > 1.3e7;
 }
 static size_t attn_tc_bytes(int64_t D) {
     return static_cast<size_t>(sm_count()) * 4 * TC_ROWS * (static_cast<size_t>(D) * sizeof(float) + sizeof(float2));

@@ -18,7 +18,6 @@
 
 namespace bt {
 
-
 struct EvictParams {
     const float* mass;
     int64_t mass_sb, mass_sh;
