@@ -1,4 +1,4 @@
-// The 16-bit kernel of bt_tree_attention for up to 16 rows per key/value head (one token with grouped heads, small trees):
+// The 16-bit kernel of bt_tree_attention for few rows per key/value head, 16 at a time (one token with grouped heads, small trees):
 // bound by HBM, so it is built around the loads.
 //
 // A CTA is four warps, and every warp is a pipeline of its own: it copies 16 slots of keys and values at a time into its
@@ -12,7 +12,9 @@
 // The weights are rounded to the cache's type for the second product (relative 2^-8 / 2^-11 at most each, their sum is
 // taken before the rounding); everything else stays float32.
 //
-// 32 sequences of 601 to 2303 slots, 20 heads, head size 128, bf16: 90 us with the join, 5.3 TB/s (a plain copy: 6.53).
+// 32 sequences of 601 to 2303 slots, 20 heads, head size 128, bf16: 90 us with the join, 5.3 TB/s (a plain copy: 6.53).  Head
+// sizes between those it is built for are padded with zeros in the ring: 8 x 4090 slots, 32 heads over 8, head size 80: 38 us,
+// on the CUDA cores 143 us.
 #pragma once
 
 #include "cache_attention.cuh"
@@ -81,11 +83,13 @@ __device__ __forceinline__ uint32_t finite_only(uint32_t w) {      // infinities
     return w;
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(AS_WARPS * 32, 2) attn_stream_kernel(const AttnParams p) {
+// FULL: the head size is D; otherwise it is a smaller multiple of 8, and the columns behind it are zeros in the ring.
+template <typename T, int D, bool FULL>
+__global__ void __launch_bounds__(AS_WARPS * 32, D <= 128 ? 2 : 1) attn_stream_kernel(const AttnParams p) {
     constexpr int PITCH = as_pitch<D>(), STAGE = as_stage_bytes<D>(), CHUNKS = D / 8, V_AT = AS_SLOTS * PITCH;
     constexpr int TILES = D / 8;                                   // n8 tiles of the output
-    static_assert(D % 32 == 0 && D <= 128, "head sizes of this kernel");
+    static_assert(D % 32 == 0 && D <= 256, "head sizes of this kernel");
+    const int width = FULL ? D : p.D;
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     float2* s_ml = reinterpret_cast<float2*>(smem + AS_WARPS * AS_STAGES * STAGE);       // [warps][rows]
@@ -114,10 +118,11 @@ __global__ void __launch_bounds__(AS_WARPS * 32, 2) attn_stream_kernel(const Att
 #pragma unroll
             for (int i = 0; i < AS_SLOTS * CHUNKS / 32; ++i) {
                 const int idx = i * 32 + lane, row = idx / CHUNKS, chunk = idx % CHUNKS;
-                const bool on = n0 + row < last;
-                const int64_t n = on ? n0 + row : first;           // a valid address for the slots that are only zeros
-                cp_async16(stage + row * PITCH + ((chunk ^ ((row & 1) << 2)) << 4), kbase + n * p.ks + chunk * 8, on);
-                cp_async16(stage + V_AT + row * PITCH + ((chunk ^ (((row >> 1) & 3) << 1)) << 4), vbase + n * p.vs + chunk * 8, on);
+                const bool on = n0 + row < last && chunk * 8 < width;
+                const int64_t n = on ? n0 + row : first;           // a valid address for what is only zeros
+                const int col = FULL || on ? chunk * 8 : 0;
+                cp_async16(stage + row * PITCH + ((chunk ^ ((row & 1) << 2)) << 4), kbase + n * p.ks + col, on);
+                cp_async16(stage + V_AT + row * PITCH + ((chunk ^ (((row >> 1) & 3) << 1)) << 4), vbase + n * p.vs + col, on);
             }
         }
         cp_async_commit();
@@ -132,8 +137,8 @@ __global__ void __launch_bounds__(AS_WARPS * 32, 2) attn_stream_kernel(const Att
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) {
         const uint4 zero = make_uint4(0, 0, 0, 0);
-        const uint4 qx = ra < p.rows ? *reinterpret_cast<const uint4*>(attn_q_row<T>(p, b, h, ra) + (c + 4 * j) * 8) : zero;
-        const uint4 qy = rb < p.rows ? *reinterpret_cast<const uint4*>(attn_q_row<T>(p, b, h, rb) + (c + 4 * j) * 8) : zero;
+        const uint4 qx = ra < p.rows && (c + 4 * j) * 8 < width ? *reinterpret_cast<const uint4*>(attn_q_row<T>(p, b, h, ra) + (c + 4 * j) * 8) : zero;
+        const uint4 qy = rb < p.rows && (c + 4 * j) * 8 < width ? *reinterpret_cast<const uint4*>(attn_q_row<T>(p, b, h, rb) + (c + 4 * j) * 8) : zero;
         qa[j][0][0] = qx.x; qa[j][0][1] = qy.x; qa[j][0][2] = qx.y; qa[j][0][3] = qy.y;
         qa[j][1][0] = qx.z; qa[j][1][1] = qy.z; qa[j][1][2] = qx.w; qa[j][1][3] = qy.w;
     }
@@ -321,6 +326,7 @@ __global__ void __launch_bounds__(AS_WARPS * 32, 2) attn_stream_kernel(const Att
     const int rows = min(AT_ROWS, p.rows - r0);
     for (int i = threadIdx.x; i < rows * (D / 4); i += AS_WARPS * 32) {
         const int r = i / (D / 4), d = i % (D / 4) * 4;
+        if (d >= width) continue;
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         float m = -INFINITY, l = 0.0f;
         float2 ml[AS_WARPS];
@@ -339,7 +345,7 @@ __global__ void __launch_bounds__(AS_WARPS * 32, 2) attn_stream_kernel(const Att
         const int64_t row = attn_row_index(p, b, h, r0 + r);
         if (p.part_ml != nullptr && d == 0) p.part_ml[row * p.nsplit + split] = make_float2(m, l);
         if (p.nsplit > 1) {
-            *reinterpret_cast<float4*>(p.part_o + (row * p.nsplit + split) * D + d) = v;
+            *reinterpret_cast<float4*>(p.part_o + (row * p.nsplit + split) * width + d) = v;
         } else {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             T* out = attn_out_row<T>(p, b, h, r0 + r) + d;
@@ -351,17 +357,17 @@ __global__ void __launch_bounds__(AS_WARPS * 32, 2) attn_stream_kernel(const Att
     }
 }
 
-template <typename T, int D>
+template <typename T, int D, bool FULL>
 static int launch_attn_stream(const AttnParams& p, void* stream) {
     static std::atomic<size_t> granted[BT_MAX_DEVICES];
-    if (const int rc = ensure_dynamic_smem(attn_stream_kernel<T, D>, as_smem<D>(), granted)) return rc;
+    if (const int rc = ensure_dynamic_smem(attn_stream_kernel<T, D, FULL>, as_smem<D>(), granted)) return rc;
     const int64_t ctas = static_cast<int64_t>(p.B) * p.Hkv * p.row_tiles * p.nsplit;
-    return launch_early(attn_stream_kernel<T, D>, "attn_stream_kernel", dim3(static_cast<unsigned>(ctas)), AS_WARPS * 32, as_smem<D>(), stream, p);
+    return launch_early(attn_stream_kernel<T, D, FULL>, "attn_stream_kernel", dim3(static_cast<unsigned>(ctas)), AS_WARPS * 32, as_smem<D>(), stream, p);
 }
 
-// Whether this kernel can take the call: 16-bit rows of a head size it is built for, every row on a 16-byte boundary.
+// Whether this kernel can take the call: 16-bit rows, every one on a 16-byte boundary and a multiple of 16 bytes long.
 static bool attn_stream_ok(const AttnParams& p) {
-    if ((p.D != 64 && p.D != 96 && p.D != 128)) return false;
+    if (p.D % 8 != 0) return false;
     const int64_t s[9] = {p.qb, p.qh, p.qt, p.kb, p.kh, p.ks, p.vb, p.vh, p.vs};
     for (const int64_t x : s)
         if (x % 8 != 0) return false;
@@ -370,9 +376,12 @@ static bool attn_stream_ok(const AttnParams& p) {
 
 template <typename T>
 static int launch_attn_stream_for(const AttnParams& p, void* stream) {
-    if (p.D == 64) return launch_attn_stream<T, 64>(p, stream);
-    if (p.D == 96) return launch_attn_stream<T, 96>(p, stream);
-    return launch_attn_stream<T, 128>(p, stream);
+    if (p.D == 64) return launch_attn_stream<T, 64, true>(p, stream);
+    if (p.D == 96) return launch_attn_stream<T, 96, true>(p, stream);
+    if (p.D == 128) return launch_attn_stream<T, 128, true>(p, stream);
+    if (p.D < 64) return launch_attn_stream<T, 64, false>(p, stream);
+    if (p.D < 128) return p.D < 96 ? launch_attn_stream<T, 96, false>(p, stream) : launch_attn_stream<T, 128, false>(p, stream);
+    return launch_attn_stream<T, 256, false>(p, stream);
 }
 
 }  // namespace bt

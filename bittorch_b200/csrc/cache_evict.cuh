@@ -6,12 +6,14 @@
 // stay.  Weights have few exponents, so most slots of a warp count into the same digit: every lane has a column of the
 // histogram to itself, and no two lanes ever meet in a bank.  Counts are integers, so the order of the atomics does
 // not matter.  A thread holds neighbouring slots, in registers for the whole selection unless the cache is longer than
-// a CTA's registers.  Bound by latency (four passes of one CTA), not by the 4 bytes a slot.
+// a CTA's registers.  Bound by the instructions and barriers of four passes of one CTA, not by the 4 bytes a slot: 8 heads of
+// 16387 slots 14 us, 256 heads of 8192 slots 24 us.
 //
 // compact: rows are copied in pieces of 16 bytes (less where the alignment asks for it), a row by neighbouring lanes.
 // Between two caches every row is independent.  In place, entry j goes to slot first + j <= keep[j], so a CTA takes a
 // narrow column of one head's cache (up to 64 bytes of every row) and walks the entries in blocks: all reads of a
-// block, a barrier, then its writes.  Reads of later blocks only touch slots that earlier writes do not reach.
+// block, a barrier, then its writes.  Reads of later blocks only touch slots that earlier writes do not reach.  Bound by HBM:
+// between two caches 32 x 8 heads x 4096 rows of 256 bytes 168 us, 6.4 TB/s.
 #pragma once
 
 #include "cache_common.cuh"
@@ -246,8 +248,12 @@ __global__ void __launch_bounds__(CG_THREADS) compact_gather_kernel(const Compac
     }
 }
 
-constexpr int CI_THREADS = 512;
-constexpr int CI_ROWS = 8;                                         // rows staged per thread and block
+// A step is a read of the entry, a read of the row, a barrier and a write, so what counts is the warps that are under way:
+// 32 sequences of 8 heads, 4096 of 8192 rows of 256 bytes in place: 512 threads with 8 rows each 429 us, 1024 with 8 303 us,
+// 1024 with 4 236 us, with 2 209 us (5.1 TB/s).  Columns of 32 bytes take 268 us there, of 128 bytes 232 us and twice as long
+// as these for few heads.
+constexpr int CI_THREADS = 1024;
+constexpr int CI_ROWS = 2;                                         // rows staged per thread and block
 constexpr int CI_COLS = 4;                                         // units of a column
 
 // In place: blockIdx.x = sequence, head and column, blockIdx.y = tensor (0, 1) or the mass (2, one column of one unit).
@@ -258,7 +264,7 @@ __device__ __forceinline__ void compact_column(uint8_t* base, int64_t stride, in
     const int lanes = cols <= 1 ? 1 : cols <= 2 ? 2 : 4;           // threads of a row
     const int col = tid % lanes, per = CI_THREADS / lanes;         // rows per pass
     U v[CI_ROWS];
-    int64_t at[CI_ROWS];
+    int at[CI_ROWS];
     for (int64_t j0 = 0; j0 < count; j0 += static_cast<int64_t>(per) * CI_ROWS) {
 #pragma unroll
         for (int i = 0; i < CI_ROWS; ++i) {
@@ -268,7 +274,7 @@ __device__ __forceinline__ void compact_column(uint8_t* base, int64_t stride, in
             const int64_t from = keep[j], to = first + j;
             if (from < 0 || from >= S || to < 0 || to >= S || from == to) continue;
             v[i] = *reinterpret_cast<const U*>(base + from * stride + (c0 + col) * sizeof(U));
-            at[i] = to;
+            at[i] = static_cast<int>(to);
         }
         __syncthreads();                                           // every read of this block, before its writes
 #pragma unroll
@@ -278,7 +284,7 @@ __device__ __forceinline__ void compact_column(uint8_t* base, int64_t stride, in
 }
 
 template <typename U>
-__global__ void __launch_bounds__(CI_THREADS) compact_inplace_kernel(const CompactParams p) {
+__global__ void __launch_bounds__(CI_THREADS, 2) compact_inplace_kernel(const CompactParams p) {
     const int columns = (p.units + CI_COLS - 1) / CI_COLS;
     const int64_t bh = blockIdx.x / columns;
     const int c0 = static_cast<int>(blockIdx.x % columns) * CI_COLS;

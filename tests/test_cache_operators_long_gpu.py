@@ -132,3 +132,12 @@ def test_two_streams_and_a_replayed_graph_over_long_caches():
     torch.cuda.synchronize()
     for _, out in graphs:
         assert all(torch.equal(a, c) for a, c in zip(out, want))
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("d", [8, 16, 40, 72, 88, 104, 120, 136, 192, 248, 256])
+def test_head_sizes(d, dtype):
+    """Head sizes between and beyond the ones that a kernel is built for: rows padded with zeros."""
+    _attention_case(2, 8, 2, 1, 310, d, [300, 64], dtype)
+    _attention_case(2, 4, 2, 9, 310, d, [301, 1], dtype, "each", stretch=2.0)
+    _attention_case(1, 6, 1, 4, 150, d, [140], dtype, "one", "bshd", with_mass=True)
