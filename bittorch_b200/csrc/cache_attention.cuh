@@ -9,8 +9,8 @@
 //
 // This file: the kernel for every type, head size and alignment (attn_split_kernel), in float32 on the CUDA cores,
 // and the join.  16 rows x 32 slots per step: each thread owns the scores of one slot for four rows, then four
-// rows x four columns of the output.  Bound by shared-memory reads of the two products; the 16-bit kernels beside it
-// take over where the tensor cores can.
+// rows x four columns of the output.  Bound by shared-memory reads of the two products; the kernels of the files beside it
+// take the calls whose rows can be read in vectors, this one what is left.
 #pragma once
 
 #include "cache_common.cuh"
@@ -365,12 +365,16 @@ static AttnPlan attn_plan(int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t 
     return a;
 }
 
-// cache_attention_stream.cuh
+// cache_attention_float.cuh, cache_attention_stream.cuh
+static bool attn_float_ok(const AttnParams& p);
+static int launch_attn_float(const AttnParams& p, void* stream);
 static bool attn_stream_ok(const AttnParams& p);
 template <typename T> static int launch_attn_stream_for(const AttnParams& p, void* stream);
 
 template <typename T>
 static int launch_attn_split(const AttnParams& p, void* stream) {
+    if constexpr (sizeof(T) == 4)
+        if (attn_float_ok(p)) return launch_attn_float(p, stream);
 #ifndef BT_SIMT_HOST
     if constexpr (sizeof(T) == 2)
         if (attn_stream_ok(p)) return launch_attn_stream_for<T>(p, stream);
@@ -456,3 +460,5 @@ extern "C" int bt_tree_attention(const void* q, const void* k, const void* v, in
     if (dtype == BT_F16) return launch_attention<__half>(p, plan, stream);
     return launch_attention<__nv_bfloat16>(p, plan, stream);
 }
+
+#include "cache_attention_float.cuh"
