@@ -2,7 +2,9 @@
 //
 // Within a beam the candidates rank by their logits, so one pass over the logits is enough: beam_scan gives every CTA
 // one piece of a row, held in registers, and leaves the piece's maximum, its sum of exponentials and its n largest
-// logits; beam_join makes the log-sums and ranks the survivors of all beams in float64.  Bound by HBM (the logits).
+// logits; beam_join makes the log-sums and ranks the survivors of all beams in float64.  32 x 8 rows of 100003 16-bit logits:
+// scan 30 us, join 11 us (a copy's time for the logits is 7.8 us): bound by the selection's instructions in the scan and by
+// the float64 exponentials and logarithms in the join.
 //
 // The n largest of a piece: 16 or 64 groups of threads have a maximum each, and the n-th of those bounds the
 // n-th of the piece from below.  What is not below it is collected and ranked by counting: with independent logits a
