@@ -8,7 +8,8 @@
 //   S = Q K^T   tcgen05.mma, both operands in shared memory, 128 columns of TMEM that the streams use in turn
 //   weights     a row's 128 scores in its thread's registers; the reference point of the exponentials moves only when a
 //               score exceeds it by 2^8 (the sums stay far from overflow, and the output is almost never rescaled);
-//               the weights, rounded to the cache's type (relative 2^-8 / 2^-11 at most), go to the stream's place in TMEM
+//               the weights, rounded to the cache's type (relative 2^-8 / 2^-11 at most; in fp16 those
+//               below 2^-14 by up to 2^-25), go to the stream's place in TMEM
 //   O += P V    tcgen05.mma with P from TMEM, V as it lies in the cache (its columns contiguous)
 //
 // Work is dealt out in blocks of 128 slots: the blocks of all pairs of tiles of all sequences form one line, and every
