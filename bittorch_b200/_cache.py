@@ -96,6 +96,12 @@ def _plain_memory(t: Tensor) -> bool:
     return True
 
 
+def _rows(t: Tensor) -> Tensor:
+    """``t`` with the elements of its last dimension side by side: itself, or a copy.  Plans and calls both go by it, so that
+    strides and pointer are of one tensor (a single element lies beside itself whatever its stride says)."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
 def _call(index: int, fn, *args) -> None:
     """Enqueue on the current stream of device ``index``."""
     if index == torch._C._cuda_getDevice():
@@ -186,8 +192,7 @@ def _attention_plan(q_sig, k_sig, v_sig, len_sig, tree_sig, scale, mass_sig, out
     if index < 0:
         return None
     out_strides = (t * h * d, d, h * d, 1) if out is None else out.stride()      # [B, T, H * D]: as the next projection reads it
-    q_strides = q.stride()[:3] if q.stride(3) == 1 or d == 1 else q.contiguous().stride()[:3]
-    strides = _TWELVE(*q_strides, *k.stride()[:3], *v.stride()[:3], *out_strides[:3])
+    strides = _TWELVE(*_rows(q).stride()[:3], *k.stride()[:3], *v.stride()[:3], *out_strides[:3])
     code = _DT[q.dtype]
     sizes = (b, h, hkv, t, s, d)
     with torch.cuda.device(index):                     # the workspace depends on the device's SM count
@@ -207,8 +212,7 @@ def tree_attention(q: Tensor, k: Tensor, v: Tensor, lengths: Tensor, tree: Optio
     if out is not None and out.untyped_storage().data_ptr() in (q.untyped_storage().data_ptr(), k.untyped_storage().data_ptr(),
                                                                 v.untyped_storage().data_ptr()):
         _fail("out must be other memory than the queries and the cache")
-    if q.stride(3) != 1:
-        q = q.contiguous()
+    q = _rows(q)
     if tree is not None and not tree.is_contiguous():
         tree = tree.contiguous()
     dev = q.device
@@ -274,7 +278,7 @@ def _compact_plan(k_sig, v_sig, keep_sig, counts_sig, first_sig, mass_sig, out_s
     if not (_plain_memory(k_out) and _plain_memory(v_out) and (mass_out is None or _plain_memory(mass_out))):
         _fail("compact_cache: what is written must share no memory with itself")
     n = keep.shape[2]
-    keep_strides = keep.stride() if keep.stride(2) == 1 or n == 1 else keep.contiguous().stride()
+    keep_strides = _rows(keep).stride()
     strides = _TWELVE(*k.stride()[:3], *v.stride()[:3], *k_out.stride()[:3], *v_out.stride()[:3])
     mass_strides = None if mass is None else _FOUR(*mass.stride()[:2], *mass_out.stride()[:2])
     return (_DT[k.dtype], b, hkv, s, s_out, d, strides), (keep_strides[0], keep_strides[1] if keep.shape[1] == hkv else 0, n), mass_strides
@@ -294,8 +298,7 @@ def compact_cache(k: Tensor, v: Tensor, keep: Tensor, counts: Tensor, first: Opt
     elif k.data_ptr() == v.data_ptr():
         _fail("keys and values that are the same memory cannot be compacted in place")
     index = _same_device("compact_cache", k, v, k_out, v_out, keep, counts, first, mass, mass_out)
-    if keep.stride(2) != 1:
-        keep = keep.contiguous()
+    keep = _rows(keep)
     counts = counts.contiguous()
     first = None if first is None else first.contiguous()
     _call(index, _compact_cache, k.data_ptr(), v.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), *head, keep.data_ptr(), *tail,
@@ -367,8 +370,7 @@ def _beam_plan(logits_sig, scores_sig, select, finished_sig, end_token):
         if not 0 <= end_token < vocab:
             _fail(f"end_token {end_token} is outside the vocabulary of {vocab}")
     code = _DT[logits.dtype]
-    strides = logits.stride()[:2] if logits.stride(2) == 1 or vocab == 1 else logits.contiguous().stride()[:2]
-    return (code, b, w, vocab, *strides), n, _beam_select_workspace(b, w, vocab, code, n)
+    return (code, b, w, vocab, *_rows(logits).stride()[:2]), n, _beam_select_workspace(b, w, vocab, code, n)
 
 
 def beam_select(logits: Tensor, scores: Tensor, select: Optional[int], finished: Optional[Tensor],
@@ -377,8 +379,7 @@ def beam_select(logits: Tensor, scores: Tensor, select: Optional[int], finished:
     if torch.is_grad_enabled():
         _no_gradient("beam_select", logits, scores)
     index = _same_device("beam_select", logits, scores, finished)
-    if logits.stride(2) != 1:
-        logits = logits.contiguous()
+    logits = _rows(logits)
     if not scores.is_contiguous():
         scores = scores.contiguous()
     if finished is not None and not finished.is_contiguous():
