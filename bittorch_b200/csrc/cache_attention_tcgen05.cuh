@@ -265,7 +265,12 @@ struct TcBars {
     uint64_t s_full[2];                                            // scores -> stream: they are there
     uint64_t s_read[2];                                            // stream -> scores: they are in registers, the buffer is free
     uint64_t p_full[2];                                            // stream -> outputs: weights are in place, output rescaled
-    uint64_t v_checked;                                            // first stream -> second: values that both multiply have been looked through
+    // First stream -> second: values that both multiply have been looked through.  Two, by turns: the scores of the first
+    // stream's next block need the second only to have read its own, so it may look through the values of that block
+    // before a warp of the second has waited for those of this one; with one barrier both phases would have passed then,
+    // and a wait by parity would not see it.  No further: the block after that one needs the second stream's next scores
+    // to have been read, which every warp does after this wait.
+    uint64_t v_checked[2];
     uint64_t pv_done[2];                                           // outputs -> stream: they have been multiplied
 };
 
@@ -318,8 +323,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             mbar_init(&bar.s_read[x], TC_ROWS);
             mbar_init(&bar.p_full[x], TC_ROWS);
             mbar_init(&bar.pv_done[x], 1);
+            mbar_init(&bar.v_checked[x], TC_ROWS);
         }
-        mbar_init(&bar.v_checked, TC_ROWS);
         s_abort_storage = 0;
         s_odd = 0;
         mbar_fence_init();
@@ -428,7 +433,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
         const int x = (warp - 2) >> 2, row = (warp & 3) * 32 + lane;   // a warp can reach the TMEM lanes of its number mod 4
         const uint32_t quarter = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t t_s = tmem + quarter, t_p = t_s + TC_WEIGHTS + x * 64, t_o = t_s + TC_OUTPUT + x * 128;
-        uint32_t n_s = 0, n_pv = 0, n_checked = 0;
+        uint32_t n_s = 0, n_pv = 0, n_checked = 0;                     // n_checked: blocks whose values the streams look through together
         bool ok = true;
         uint8_t* stage = s_stage + (warp - 2) * TC_STAGE;
         uint4* bits = s_bits + x * TC_NODES;
@@ -571,9 +576,13 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     if (bad) *reinterpret_cast<volatile int*>(&s_odd) = 1;
                     fence_proxy_async_smem();
                     __syncwarp();
-                    if (c.streams == 2 && !c.own) mbar_arrive(&bar.v_checked);
+                    if (c.streams == 2 && !c.own) {
+                        mbar_arrive(&bar.v_checked[n_checked & 1]);
+                        ++n_checked;
+                    }
                 } else if (tail) {
-                    if (!wait_or_abort_warp(&bar.v_checked, n_checked++ & 1, s_abort)) { ok = false; break; }
+                    if (!wait_or_abort_warp(&bar.v_checked[n_checked & 1], (n_checked >> 1) & 1, s_abort)) { ok = false; break; }
+                    ++n_checked;
                 }
                 tmem_st_wait();
                 tc_fence_before();
