@@ -255,9 +255,6 @@ __device__ __forceinline__ constexpr uint32_t tc_idesc(int n, bool b_columns_con
     return (1u << 4) | (fmt << 7) | (fmt << 10) | ((b_columns_contiguous ? 1u : 0u) << 16) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(TC_ROWS >> 4) << 24);
 }
 
-// Barrier over the 128 threads of a stream
-__device__ __forceinline__ void named_barrier_of_stream(int x) { asm volatile("bar.sync %0, 128;" ::"r"(x + 1) : "memory"); }
-
 struct TcBars {
     uint64_t full[TC_SLOTS];                                       // TMA -> products
     uint64_t empty[TC_SLOTS];                                      // products -> TMA
@@ -272,6 +269,8 @@ struct TcBars {
     // to have been read, which every warp does after this wait.
     uint64_t v_checked[2];
     uint64_t pv_done[2];                                           // outputs -> stream: they have been multiplied
+    uint64_t bits[2];                                              // among the threads of a stream, twice a piece: its tree's old bits are free, the new ones there
+    uint64_t drained[2];                                           // at the end: the products that a warp has issued have been made
 };
 
 // Copies the queries of a tile into shared memory, asynchronously: each warp its own 32 rows, neighbouring lanes a row.
@@ -324,6 +323,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             mbar_init(&bar.p_full[x], TC_ROWS);
             mbar_init(&bar.pv_done[x], 1);
             mbar_init(&bar.v_checked[x], TC_ROWS);
+            mbar_init(&bar.bits[x], TC_ROWS);
+            mbar_init(&bar.drained[x], 1);
         }
         s_abort_storage = 0;
         s_odd = 0;
@@ -428,6 +429,10 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     __syncwarp();
                 }
         }
+        // What was issued must end before the tensor memory is freed, whichever role gave up (else it has, or is about to).
+        if (elect_one_lane()) umma_commit(&bar.drained[values]);
+        __syncwarp();
+        mbar_wait_bounded(&bar.drained[values], 0);
     } else {
         // ================= streams: one thread per row =================
         const int x = (warp - 2) >> 2, row = (warp & 3) * 32 + lane;   // a warp can reach the TMEM lanes of its number mod 4
@@ -442,6 +447,12 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             cp_async_wait<0>();
             fence_proxy_async_smem();
             mbar_arrive(&bar.q_full[x]);
+        };
+        // Every wait of the streams is one that gives up when another role has, their own barrier among them: a warp that
+        // has left does not come to it.
+        auto stream_together = [&](uint32_t parity) {
+            mbar_arrive(&bar.bits[x]);
+            return wait_or_abort_warp(&bar.bits[x], parity, s_abort);
         };
         int turn = 0;
         // Where the stream is lives in shared memory: the registers are for the scores.
@@ -474,7 +485,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             const bool table = p.a.tree != nullptr && p.a.T <= TC_NODES;
             if (table && c.k1 * TC_KEYS > c.len) {                 // this piece reaches the new tokens: a tree row as 128 bits
                 const uint8_t* tree = p.a.tree + c.b * p.a.tree_sb;
-                named_barrier_of_stream(x);                        // the last piece's bits are no longer needed
+                if (!stream_together(0)) { ok = false; break; }    // the last piece's bits are no longer needed
 #pragma unroll 4
                 for (int i = row >> 5; i < p.a.T; i += 4) {
                     uint32_t w[4];
@@ -485,7 +496,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     }
                     if (lane == 0) bits[i] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
-                named_barrier_of_stream(x);
+                if (!stream_together(1)) { ok = false; break; }
             }
             float m = -INFINITY, l = 0.0f;
             for (int k = c.k0; k < c.k1; ++k) {
@@ -646,6 +657,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             }
             tc_fence_before();                                     // before the next piece's weights, which say that the output may be overwritten
         }
+        tmem_st_wait();                                            // weights on their way when a wait ran out
     }
     tc_fence_before();
     __syncthreads();

@@ -152,3 +152,20 @@ def test_the_search_finds_a_lapped_wait():
     """With one barrier the first stream may arrive for a second block before a warp of the second has looked for the first."""
     assert deadlocks([(3, 2)], 1) and deadlocks([(1, 1), (1, 1), (1, 1)], 1)
     assert not deadlocks([(3, 1)], 1)
+
+
+def test_every_wait_of_the_kernel_gives_up():
+    """A role whose wait runs out leaves for the end of the kernel; whoever waits for it must give up too.  So no wait between
+    the CTA's first barrier and its last is one that does not: no barrier by number, no polling without a limit."""
+    text = open(SOURCE).read()
+    kernel = text[text.index("attn_tc_kernel(const __grid_constant__"):text.index("// Adds up the pieces")]
+    assert kernel.count("__syncthreads();") == 2                            # every thread comes to both, whatever it has given up
+    assert not re.search(r"bar\.sync|barrier\.(cta\.)?sync|named_barrier", text)
+    assert not re.search(r"while\s*\(\s*!\s*mbar_try_wait", text)
+    assert set(re.findall(r"\b(\w*wait\w*)\(", kernel)) <= {"wait_or_abort", "wait_or_abort_warp", "mbar_wait_bounded", "tmem_ld_wait", "tmem_st_wait",
+                                                             "pdl_wait", "cp_async_wait"}
+    # each wait that gives up is looked at
+    for line in kernel.splitlines():
+        for found in re.finditer(r"wait_or_abort(_warp)?\(|stream_together\([01]\)", line):
+            before = line[:found.start()].rstrip()
+            assert before.endswith(("!", "ok = ok &&", "|| !", "return")), line
