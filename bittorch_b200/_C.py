@@ -22,7 +22,7 @@ from . import _build
 
 BT_F32, BT_F16, BT_BF16, BT_F64 = 0, 1, 2, 3
 LAUNCH_DEFAULT, LAUNCH_WEIGHTS_JUST_WRITTEN = 0, 1
-TUNE_GEMM_PAIR, TUNE_GEMM_BN, TUNE_GEMM_SPLIT, TUNE_GEMV_SPLIT = 0, 1, 2, 3
+TUNE_GEMM_PAIR, TUNE_GEMM_BN, TUNE_GEMM_SPLIT, TUNE_GEMV_SPLIT, TUNE_ATTENTION_GIVE_UP = 0, 1, 2, 3, 4
 AMAX_SLOTS = 8           # words per row of the row-maximum buffers of gemv_tiled_chained
 GEMV_MAX_M = 16          # largest batch the decode kernels accept
 DECODE_MAX_M = 4         # batches up to here run the decode kernel; above it the tensor-core kernel is faster

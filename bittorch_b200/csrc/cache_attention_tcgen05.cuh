@@ -58,6 +58,7 @@ struct AttnTcParams {
     float scale2;                                                  // scale * log2(e), not negative
     float* part_o;                                                 // [CTA][2][stream][D][128]: rows vary fastest, as the threads do
     float2* part_ml;                                               // [CTA][2][stream][128]
+    int give_up;                                                   // self-test: every CTA's TMA role leaves after so many tiles, as if a wait had run out; -1: never
 };
 
 // A piece of one pair's line of blocks
@@ -290,6 +291,20 @@ __device__ __noinline__ void tc_fetch_queries(const AttnTcParams& p, int b, int 
     cp_async_commit();
 }
 
+// What a stream leaves of a piece that it cannot finish because a wait has run out: NaN, in the output or in the workspace (from
+// where the join carries them on), so that nothing that was never written passes for a result.
+template <typename T, int D>
+__device__ __noinline__ void tc_leave_nan(const AttnTcParams& p, const TcPiece& c, int x, int row) {
+    const int item = c.pair * 2 + x, h = item / p.tiles, r = (item - h * p.tiles) * TC_ROWS + row;
+    const float nan = __int_as_float(0x7fffffff);
+    if (c.k0 > 0 || c.k1 < c.blocks) {
+        p.part_ml[((static_cast<int64_t>(blockIdx.x) * 2 + (c.k0 > 0 ? 0 : 1)) * 2 + x) * TC_ROWS + row] = make_float2(nan, nan);
+    } else if (r < p.a.rows) {
+        T* out = attn_out_row<T>(p.a, c.b, h, r);
+        for (int d = 0; d < D; ++d) out[d] = from_float<T>(nan);
+    }
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(TC_THREADS, 1)
 attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnTcParams p) {
@@ -356,6 +371,11 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             uint32_t pos = 0;
             auto load = [&](const CUtensorMap* map, int head, int block) {
                 const uint32_t s = pos % TC_SLOTS;
+                if (pos == static_cast<uint32_t>(p.give_up)) {
+                    report_wait_timeout();
+                    *s_abort = 1;
+                    return false;
+                }
                 if (!wait_or_abort(&bar.empty[s], ((pos / TC_SLOTS) & 1) ^ 1, s_abort)) return false;
                 mbar_expect_tx(&bar.full[s], TILE);
 #pragma unroll
@@ -485,7 +505,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             const bool table = p.a.tree != nullptr && p.a.T <= TC_NODES;
             if (table && c.k1 * TC_KEYS > c.len) {                 // this piece reaches the new tokens: a tree row as 128 bits
                 const uint8_t* tree = p.a.tree + c.b * p.a.tree_sb;
-                if (!stream_together(0)) { ok = false; break; }    // the last piece's bits are no longer needed
+                if (!stream_together(0)) { ok = false; more = advance(); break; }      // the last piece's bits are no longer needed
 #pragma unroll 4
                 for (int i = row >> 5; i < p.a.T; i += 4) {
                     uint32_t w[4];
@@ -496,7 +516,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                     }
                     if (lane == 0) bits[i] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
-                if (!stream_together(1)) { ok = false; break; }
+                if (!stream_together(1)) { ok = false; more = advance(); break; }
             }
             float m = -INFINITY, l = 0.0f;
             for (int k = c.k0; k < c.k1; ++k) {
@@ -599,7 +619,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
                 tc_fence_before();
                 mbar_arrive(&bar.p_full[x]);
             }
-            if (!ok) break;
+            if (!ok) { more = advance(); break; }
             more = advance();                                      // the last product with these queries is done
             if (more) {
                 fetch_queries(s_piece[warp - 2][turn ^ 1]);
@@ -657,6 +677,14 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
             }
             tc_fence_before();                                     // before the next piece's weights, which say that the output may be overwritten
         }
+        if (!ok)                                                   // the piece that was under way, and those after it
+            while (true) {
+                tc_leave_nan<T, D>(p, s_piece[warp - 2][turn], x, row);
+                if (!more) break;
+                turn ^= 1;
+                more = advance();
+            }
+        __syncwarp();
         tmem_st_wait();                                            // weights on their way when a wait ran out
     }
     tc_fence_before();
@@ -786,6 +814,7 @@ static int launch_attn_tc(const AttnParams& a, int dtype, float scale, void* wor
     p.pairs = ceil_div(p.items, 2);
     p.scale2 = std::max(scale * 1.4426950408889634f, 1e-30f);      // not 0: masked scores are -infinity
     const int ctas = sm_count();
+    p.give_up = tuning(BT_TUNE_ATTENTION_GIVE_UP);
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<size_t>(ctas) * 4 * TC_ROWS * D);
     static std::atomic<size_t> granted[BT_MAX_DEVICES];

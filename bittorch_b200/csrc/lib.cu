@@ -38,9 +38,9 @@ static std::once_flag g_tuning_once;
 
 static void tuning_init() {
     static const char* const env_names[BT_TUNE_COUNT] = {"BITTORCH_B200_GEMM_PAIR", "BITTORCH_B200_GEMM_BN",
-                                                         "BITTORCH_B200_GEMM_SPLIT", "BITTORCH_B200_GEMV_SPLIT"};
+                                                         "BITTORCH_B200_GEMM_SPLIT", "BITTORCH_B200_GEMV_SPLIT", nullptr};
     for (int k = 0; k < BT_TUNE_COUNT; ++k) {
-        const char* e = std::getenv(env_names[k]);
+        const char* e = env_names[k] != nullptr ? std::getenv(env_names[k]) : nullptr;
         g_tuning[k].store(e != nullptr ? std::atoi(e) : -1, std::memory_order_relaxed);
     }
 }

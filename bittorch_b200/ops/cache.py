@@ -66,6 +66,9 @@ def tree_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, lengths: Tensor,
     a tree per sequence; None: j <= i).  T = 1 without a tree is plain decoding.  Query head h reads key/value head
     ``h // (H // Hkv)``.  ``scale``: D ** -0.5.  A token that sees nothing gives zeros.  Slots from S on do not exist.
 
+    Should a wait inside the kernel run out (after 2 s: a fault of the kernel or the device), what it could not write is NaN,
+    and ``_C.device_status()`` says so.
+
     ``mass`` float32 [B, Hkv, S]: every slot's attention weight, summed over the heads of its group and the T tokens, is
     added to it in place (what ``evict_cache`` goes by)."""
     return _binding().tree_attention(q, k_cache, v_cache, lengths, tree, scale, mass, out)

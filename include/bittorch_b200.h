@@ -60,12 +60,13 @@ extern "C" {
 
 /* Kernel-selection overrides for tests and tuning, bt_set_tuning(knob, value); value -1
  * (the default) lets the library choose.  Each knob's initial value comes from the
- * environment variable named beside it, read once. */
+ * environment variable named beside it (where one is), read once. */
 #define BT_TUNE_GEMM_PAIR 0   /* BITTORCH_B200_GEMM_PAIR : 1 / 0 force the CTA-pair GEMM on / off */
 #define BT_TUNE_GEMM_BN 1     /* BITTORCH_B200_GEMM_BN   : 64 / 128 / 256 output-tile width */
 #define BT_TUNE_GEMM_SPLIT 2  /* BITTORCH_B200_GEMM_SPLIT: 1 / 2 / 4 / 8 K split of the narrow-batch GEMM */
 #define BT_TUNE_GEMV_SPLIT 3  /* BITTORCH_B200_GEMV_SPLIT: 1 / 2 / 4 / 8 K split of bt_gemv_packed_i8 */
-#define BT_TUNE_COUNT 4
+#define BT_TUNE_ATTENTION_GIVE_UP 4   /* self-test: bt_tree_attention's tensor-memory kernel gives up after so many tiles (set by bt_set_tuning only) */
+#define BT_TUNE_COUNT 5
 
 /* Largest M handled by the decode (GEMV) kernels. */
 #define BT_GEMV_MAX_M 16

@@ -38,7 +38,8 @@ extern "C" {
  * Query head h reads key/value head h / (H / Hkv).  A token that sees nothing gives
  * zeros.  Slots that no token sees are never read into a result, whatever they hold.
  * Sums and softmax statistics are float32; with 16-bit types the weights are rounded to
- * that type for the product with the values.
+ * that type for the product with the values.  Should a wait of the kernel run out (2 s), what
+ * it could not write is NaN and bt_device_status() says BT_ERR_DEVICE_WAIT.
  *
  * q [B,H,T,D], k and v [B,Hkv,S,D], out [B,H,T,D], all of `dtype`;
  * strides  host int64[12]: q (b,h,t), k (b,h,s), v (b,h,s), out (b,h,t)

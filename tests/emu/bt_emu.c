@@ -129,7 +129,7 @@ int bt_version(void) { return 100; }
 const char* bt_last_error(void) { return g_error; }
 
 static int g_status = 0;
-static int g_tuning[BT_TUNE_COUNT] = {-1, -1, -1, -1};
+static int g_tuning[BT_TUNE_COUNT] = {-1, -1, -1, -1, -1};
 
 int bt_device_status(int* status_host, void* stream) {
     (void)stream;

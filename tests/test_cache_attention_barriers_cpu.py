@@ -163,7 +163,7 @@ def test_every_wait_of_the_kernel_gives_up():
     assert not re.search(r"bar\.sync|barrier\.(cta\.)?sync|named_barrier", text)
     assert not re.search(r"while\s*\(\s*!\s*mbar_try_wait", text)
     assert set(re.findall(r"\b(\w*wait\w*)\(", kernel)) <= {"wait_or_abort", "wait_or_abort_warp", "mbar_wait_bounded", "tmem_ld_wait", "tmem_st_wait",
-                                                             "pdl_wait", "cp_async_wait"}
+                                                             "pdl_wait", "cp_async_wait", "report_wait_timeout"}
     # each wait that gives up is looked at
     for line in kernel.splitlines():
         for found in re.finditer(r"wait_or_abort(_warp)?\(|stream_together\([01]\)", line):

@@ -43,3 +43,36 @@ def test_new_tokens_in_neighbouring_blocks(b, h, hkv, t, s, d, lens, dtype):
     for _ in range(50):
         assert torch.equal(ops.tree_attention(q, k, v, lengths, tree), got)
     assert _C.device_status() == 0
+
+
+@pytest.mark.parametrize("tiles", [0, 1, 5, 12])
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float16, 64)])
+def test_a_call_whose_wait_runs_out_leaves_nan_and_a_status(dtype, d, tiles):
+    """The give-up path: the role that brings the tiles leaves after some of them, as it does when its wait runs out, and all
+    others follow (every wait of theirs has a limit).  What was finished before is right, the rest is NaN, nothing is left
+    unwritten, and the next call is as ever."""
+    from bittorch_b200 import _C
+
+    ops = _ops()
+    b, h, hkv, t, s = 24, 32, 8, 61, 2304                                   # about 19 places of the line for each CTA
+    _large(b, h, hkv, t, s, d)
+    g = torch.Generator().manual_seed(tiles)
+    k, v = (torch.randn(b, hkv, s, d, generator=g).to(dtype).cuda() for _ in range(2))
+    q = torch.randn(b, h, t, d, generator=g).to(dtype).cuda()
+    tree = (torch.rand(t, t, generator=g) < 0.5).cuda()
+    lengths = torch.tensor([100, 2200, 0, 1300, 64, 2243] * 4).cuda()
+    clean = ops.tree_attention(q, k, v, lengths, tree)
+    assert _C.device_status() == 0
+    out = torch.full((b, h, t, d), 7.0, dtype=dtype, device="cuda")
+    _C.set_tuning(_C.TUNE_ATTENTION_GIVE_UP, tiles)
+    try:
+        ops.tree_attention(q, k, v, lengths, tree, out=out)
+        torch.cuda.synchronize()
+    finally:
+        _C.set_tuning(_C.TUNE_ATTENTION_GIVE_UP, -1)
+    assert _C.device_status() == 4
+    lost = out.isnan().any(-1)
+    assert bool(lost.any()) and bool(out.isnan().all(-1)[lost].all())
+    assert bool(lost.all()) or tiles > 0
+    assert torch.equal(out[~lost], clean[~lost])
+    assert torch.equal(ops.tree_attention(q, k, v, lengths, tree), clean) and _C.device_status() == 0
