@@ -96,6 +96,62 @@ def _plain_memory(t: Tensor) -> bool:
     return True
 
 
+def _span(shape, stride, dtype: torch.dtype) -> int:
+    """Bytes from the first element of a tensor to behind its last."""
+    return (1 + sum((n - 1) * st for n, st in zip(shape, stride))) * dtype.itemsize
+
+
+@functools.lru_cache(maxsize=1024)
+def _meet(a_sig, b_sig, distance: int) -> bool:
+    """Whether tensors of these shapes, strides and types have a byte in common, the second ``distance`` bytes behind the
+    first.  A byte of the first less one of the second is a sum of steps, each taken a bounded number of times; from the
+    longest step down, what is left must be within reach of the shorter ones, which for the nested strides of a tensor
+    leaves one or two numbers to try.  Layouts that take more than 4096 trials count as meeting."""
+    steps = {}
+    for (shape, stride, dtype), sign in ((a_sig, 1), (b_sig, -1)):
+        for n, st in (*zip(shape, (st * dtype.itemsize for st in stride)), (dtype.itemsize, 1)):
+            if n > 1 and st > 0:
+                low, high = steps.get(st, (0, 0))
+                steps[st] = (low - (n - 1), high) if sign < 0 else (low, high + n - 1)
+    order = sorted(steps, reverse=True)
+    reach = [0]                                            # of the steps from a place on, each counted from its lowest number
+    for st in reversed(order):
+        reach.insert(0, reach[0] + st * (steps[st][1] - steps[st][0]))
+    trials = 0
+
+    def solve(i: int, left: int) -> bool:
+        nonlocal trials
+        trials += 1
+        if trials > 4096 or left == 0:
+            return True
+        if i == len(order) or left > reach[i]:
+            return False
+        st = order[i]
+        most = min(left // st, steps[st][1] - steps[st][0])
+        least = max(0, -((reach[i + 1] - left) // st))
+        return any(solve(i + 1, left - n * st) for n in range(most, least - 1, -1))
+
+    target = distance - sum(st * low for st, (low, _) in steps.items())
+    return target >= 0 and solve(0, target)
+
+
+def _apart(a, b) -> bool:
+    """Whether two tensors, each given as (tensor, address, span in bytes), share no memory."""
+    return a[1] + a[2] <= b[1] or b[1] + b[2] <= a[1] or not _meet(_sig(a[0]), _sig(b[0]), b[1] - a[1])
+
+
+def _all_apart(written, read=()) -> bool:
+    """Whether what a call writes shares no memory with what else it writes or reads."""
+    for i, a in enumerate(written):
+        for b in written[i + 1:]:
+            if not _apart(a, b):
+                return False
+        for b in read:
+            if not _apart(a, b):
+                return False
+    return True
+
+
 def _rows(t: Tensor) -> Tensor:
     """``t`` with the elements of its last dimension side by side: itself, or a copy.  Plans and calls both go by it, so that
     strides and pointer are of one tensor (a single element lies beside itself whatever its stride says)."""
@@ -281,22 +337,26 @@ def _compact_plan(k_sig, v_sig, keep_sig, counts_sig, first_sig, mass_sig, out_s
     keep_strides = _rows(keep).stride()
     strides = _TWELVE(*k.stride()[:3], *v.stride()[:3], *k_out.stride()[:3], *v_out.stride()[:3])
     mass_strides = None if mass is None else _FOUR(*mass.stride()[:2], *mass_out.stride()[:2])
-    return (_DT[k.dtype], b, hkv, s, s_out, d, strides), (keep_strides[0], keep_strides[1] if keep.shape[1] == hkv else 0, n), mass_strides
+    spans = [tuple(_span(*sig) for sig in sigs if sig is not None) for sigs in ((k_sig, v_sig, mass_sig), out_sigs or ())]
+    return (_DT[k.dtype], b, hkv, s, s_out, d, strides), (keep_strides[0], keep_strides[1] if keep.shape[1] == hkv else 0, n), mass_strides, spans
+
+
+def _moves_apart(spans, cache, out) -> bool:
+    """Whether a compaction of ``cache`` = (keys, values[, mass]), in place or into ``out``, writes over nothing that it reads."""
+    read = [(t, t.data_ptr(), n) for t, n in zip(cache, spans[0])]
+    return _all_apart(read) if out is None else _all_apart([(t, t.data_ptr(), n) for t, n in zip(out, spans[1])], read)
 
 
 def compact_cache(k: Tensor, v: Tensor, keep: Tensor, counts: Tensor, first: Optional[Tensor], mass: Optional[Tensor],
                   out: Optional[Sequence[Tensor]]) -> None:
-    head, tail, mass_strides = _compact_plan(_sig(k), _sig(v), _sig(keep), _sig(counts), _sig(first), _sig(mass),
-                                             None if out is None else tuple(_sig(x) for x in out))
+    head, tail, mass_strides, spans = _compact_plan(_sig(k), _sig(v), _sig(keep), _sig(counts), _sig(first), _sig(mass),
+                                                    None if out is None else tuple(_sig(x) for x in out))
     k_out, v_out, mass_out = (k, v, mass) if out is None else (out[0], out[1], out[2] if mass is not None else None)
     if torch.is_grad_enabled():
         _no_gradient("compact_cache", k, v, k_out, v_out, mass, mass_out)
-    if out is not None:
-        apart = [x.data_ptr() for x in (k, v, k_out, v_out)]
-        if apart[2] in apart[:2] or apart[3] in apart[:3] or (mass is not None and mass_out.data_ptr() == mass.data_ptr()):
-            _fail("out must be other memory than the cache (leave it out to compact in place)")
-    elif k.data_ptr() == v.data_ptr():
-        _fail("keys and values that are the same memory cannot be compacted in place")
+    if not _moves_apart(spans, (k, v) if mass is None else (k, v, mass), out):
+        _fail("keys and values (and mass) that share the same memory cannot be compacted in place" if out is None else
+              "out must be other memory than the cache and share none within itself (leave it out to compact in place)")
     index = _same_device("compact_cache", k, v, k_out, v_out, keep, counts, first, mass, mass_out)
     keep = _rows(keep)
     counts = counts.contiguous()
@@ -321,21 +381,20 @@ def _evict_cache_plan(k_sig, v_sig, mass_sig, len_sig, budget, sinks, recent, ou
 def evict_cache(k: Tensor, v: Tensor, mass: Tensor, lengths: Tensor, budget: int, sinks: int, recent: int,
                 out: Optional[Sequence[Tensor]]) -> Tuple[Tensor, Tensor]:
     budget, sinks, recent = int(budget), int(sinks), int(recent)
-    (sizes, strides, lens), (head, tail, mass_strides) = _evict_cache_plan(
+    (sizes, strides, lens), (head, tail, mass_strides, spans) = _evict_cache_plan(
         _sig(k), _sig(v), _sig(mass), _sig(lengths), budget, sinks, recent, None if out is None else tuple([_sig(x) for x in out]))
     k_out, v_out, mass_out = (k, v, mass) if out is None else out
     if torch.is_grad_enabled():
         _no_gradient("evict_cache", k, v, k_out, v_out, mass, mass_out)
     k_at, v_at, mass_at = k.data_ptr(), v.data_ptr(), mass.data_ptr()
+    if not _moves_apart(spans, (k, v, mass), out):
+        _fail("keys, values and mass that share the same memory cannot be evicted from in place" if out is None else
+              "out must be other memory than the cache and share none within itself (leave it out to evict in place)")
     if out is None:
-        if k_at == v_at:
-            _fail("keys and values that are the same memory cannot be evicted from in place")
         k_to, v_to, mass_to = k_at, v_at, mass_at
         index = _same_device("evict_cache", k, v, mass, lengths)
     else:
         k_to, v_to, mass_to = k_out.data_ptr(), v_out.data_ptr(), mass_out.data_ptr()
-        if k_to in (k_at, v_at) or v_to in (k_at, v_at, k_to) or mass_to == mass_at:
-            _fail("out must be other memory than the cache (leave it out to evict in place)")
         index = _same_device("evict_cache", k, v, mass, lengths, k_out, v_out, mass_out)
     b, hkv, _ = sizes
     keep = torch.empty((b, hkv, budget), dtype=torch.int64, device=k.device)

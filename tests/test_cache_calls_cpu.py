@@ -58,3 +58,66 @@ def test_plans_take_the_strides_of_the_tensor_that_is_read(monkeypatch, shape):
         args = calls.pop()[1]
         own = args[0] == logits.data_ptr()
         assert own == (d == 1) and list(args[5:7]) == list((logits if own else logits.contiguous()).stride()[:2])
+
+
+def test_shared_memory_is_found_exactly():
+    """Every pair of random views of one buffer against the elements that they hold."""
+    import numpy as np
+    from bittorch_b200 import _cache
+
+    rng = np.random.default_rng(0)
+    found = {True: 0, False: 0}
+    for _ in range(3000):
+        pair = []
+        for _ in range(2):
+            base = torch.zeros(int(rng.integers(1, 5)), int(rng.integers(1, 5)), int(rng.integers(2, 9)), int(rng.integers(1, 7)))
+            view = base.permute(*rng.permutation(4).tolist())
+            view = view[tuple(slice(int(rng.integers(0, n)), None, int(rng.integers(1, 3))) for n in view.shape)]
+            pair.append((view.shape, view.stride(), [torch.float32, torch.bfloat16][int(rng.integers(2))], view.storage_offset()))
+        if rng.random() < 0.5:
+            pair[1] = (*pair[0][:2], pair[1][2], pair[1][3])
+        at = [x[3] * x[2].itemsize + int(rng.integers(0, 40)) * 2 for x in pair]
+        held = [set((p + x[2].itemsize * np.add.outer(sum(np.ix_(*[np.arange(n) * st for n, st in zip(x[0], x[1])])), np.zeros(1, int)).reshape(-1, 1)
+                     + np.arange(x[2].itemsize)).reshape(-1).tolist()) for p, x in zip(at, pair)]
+        want = bool(held[0] & held[1])
+        a, b = (tuple(x[:3]) for x in pair)
+        assert _cache._meet(a, b, at[1] - at[0]) == want == _cache._meet(b, a, at[0] - at[1])
+        found[want] += 1
+    assert min(found.values()) > 100
+
+
+def test_a_compaction_refuses_partly_shared_memory(monkeypatch):
+    """An output that begins some slots into the cache, keys and values that overlap; views of one buffer that hold no common
+    element are taken."""
+    g = torch.Generator().manual_seed(1)
+    with on_the_cpu(monkeypatch) as (ops, _):
+        buf = torch.randn(2, 3, 20, 8, generator=g)
+        k, v = buf[:, :, :10], torch.randn(2, 3, 10, 8, generator=g)
+        keep, counts = torch.tensor([[[1, 4, 6]]]).expand(2, 3, 3), torch.tensor([3, 2])
+        mass, lengths = torch.rand(2, 3, 10, generator=g), torch.tensor([10, 9])
+        for first in (0, 1, 9):                                             # they meet in slots first .. 9
+            with pytest.raises(RuntimeError, match="other memory"):
+                ops.compact_cache(k, v, keep, counts, out=(buf[:, :, first:first + 5], torch.empty(2, 3, 5, 8)))
+            with pytest.raises(RuntimeError, match="other memory"):
+                ops.evict_cache(k, v, mass, lengths, 5, out=(torch.empty(2, 3, 5, 8), buf[:, :, first:first + 5], torch.empty(2, 3, 5)))
+        big = torch.randn(2, 3, 9, 8, generator=g)
+        with pytest.raises(RuntimeError, match="other memory"):
+            ops.compact_cache(k, v, keep, counts, out=(big[:, :, :5], big[:, :, 4:]))
+        with pytest.raises(RuntimeError, match="same memory"):
+            ops.compact_cache(buf[:, :, :10], buf[:, :, 9:19], keep, counts)
+        with pytest.raises(RuntimeError, match="same memory"):
+            ops.evict_cache(buf[:, :, :10], buf[:, :, 9:19], mass, lengths, 5)
+        with pytest.raises(RuntimeError, match="other memory"):
+            ops.evict_cache(k, v, mass, lengths, 5, out=(torch.empty(2, 3, 5, 8), torch.empty(2, 3, 5, 8), mass[:, :, 3:8]))
+        # the two halves of one buffer, as output and as keys and values; heads and slots in turn
+        want = [k.gather(2, keep[..., None].expand(2, 3, 3, 8)), v.gather(2, keep[..., None].expand(2, 3, 3, 8))]
+        out = (buf[:, :, 10:15], torch.zeros(2, 3, 5, 8))
+        ops.compact_cache(k, v, keep, counts, out=out)
+        for x, w in zip(out, want):
+            assert torch.equal(x[0, :, :3], w[0]) and torch.equal(x[1, :, :2], w[1, :, :2])
+        pair = torch.randn(2, 10, 2, 3, 8, generator=g)
+        k, v = pair[:, :, 0].transpose(1, 2), pair[:, :, 1].transpose(1, 2)
+        want = [k.gather(2, keep[..., None].expand(2, 3, 3, 8)), v.gather(2, keep[..., None].expand(2, 3, 3, 8))]
+        ops.compact_cache(k, v, keep, counts)
+        for x, w in zip((k, v), want):
+            assert torch.equal(x[0, :, :3], w[0]) and torch.equal(x[1, :, :2], w[1, :, :2])
