@@ -253,7 +253,8 @@ def _attention_plan(q_sig, k_sig, v_sig, len_sig, tree_sig, scale, mass_sig, out
     sizes = (b, h, hkv, t, s, d)
     with torch.cuda.device(index):                     # the workspace depends on the device's SM count
         need = _tree_attention_workspace(*sizes, code, mass is not None)
-    return (code, *sizes, strides), (len64, len_stride), tree_sb, ((0, 0) if mass is None else mass.stride()[:2]), need, out_strides
+    spans = tuple(0 if sig is None else _span(*sig) for sig in (q_sig, k_sig, v_sig, mass_sig, out_sig))
+    return (code, *sizes, strides), (len64, len_stride), tree_sb, ((0, 0) if mass is None else mass.stride()[:2]), need, out_strides, spans
 
 
 def tree_attention(q: Tensor, k: Tensor, v: Tensor, lengths: Tensor, tree: Optional[Tensor], scale: Optional[float],
@@ -264,10 +265,11 @@ def tree_attention(q: Tensor, k: Tensor, v: Tensor, lengths: Tensor, tree: Optio
     if torch.is_grad_enabled():
         _no_gradient("tree_attention", q, k, v, mass, out)
     index = _same_device("tree_attention", q, k, v, lengths, tree, mass, out)
-    head, lens, tree_sb, mass_strides, need, out_strides = plan
-    if out is not None and out.untyped_storage().data_ptr() in (q.untyped_storage().data_ptr(), k.untyped_storage().data_ptr(),
-                                                                v.untyped_storage().data_ptr()):
-        _fail("out must be other memory than the queries and the cache")
+    head, lens, tree_sb, mass_strides, need, out_strides, spans = plan
+    if out is not None or mass is not None:
+        written = [(t, t.data_ptr(), n) for t, n in ((mass, spans[3]), (out, spans[4])) if t is not None]
+        if not _all_apart(written, [(t, t.data_ptr(), n) for t, n in zip((q, k, v), spans)]):
+            _fail("out and mass must be other memory than the queries and the cache, and than each other")
     q = _rows(q)
     if tree is not None and not tree.is_contiguous():
         tree = tree.contiguous()

@@ -121,3 +121,30 @@ def test_a_compaction_refuses_partly_shared_memory(monkeypatch):
         ops.compact_cache(k, v, keep, counts)
         for x, w in zip((k, v), want):
             assert torch.equal(x[0, :, :3], w[0]) and torch.equal(x[1, :, :2], w[1, :, :2])
+
+
+def test_attention_refuses_shared_memory_and_nothing_else(monkeypatch):
+    """An output beside the queries in one buffer is memory of its own; one that meets an operand is not, nor is such a mass."""
+    g = torch.Generator().manual_seed(2)
+    with on_the_cpu(monkeypatch) as (ops, _):
+        both = torch.randn(2, 3, 4, 16, generator=g)                        # queries and output in one buffer, row by row
+        q, out = both[..., :8], both[..., 8:]
+        slots = torch.randn(2, 2, 3, 9, 8, generator=g)
+        k, v = slots[0], slots[1]
+        lengths = torch.tensor([5, 2])
+        want, _, largest = ref.attention(q, k, v, lengths)
+        assert ops.tree_attention(q, k, v, lengths, out=out) is out
+        # as in the CPU tests of the kernels: 4e-6 (1 + largest) for scores and sums, one rounding
+        assert torch.allclose(out.double(), want, rtol=2.0 ** -24, atol=4e-6 * (1 + largest))
+        whole = torch.randn(2, 3, 6, 8, generator=g)
+        with pytest.raises(RuntimeError, match="other memory"):
+            ops.tree_attention(whole[:, :, :4], k, v, lengths, out=whole[:, :, 2:])
+        with pytest.raises(RuntimeError, match="other memory"):
+            ops.tree_attention(q, k, v, lengths, out=k[:, :, :4])
+        with pytest.raises(RuntimeError, match="other memory"):
+            ops.tree_attention(q, k, v, lengths, mass=v.reshape(-1)[:54].view(2, 3, 9))
+        with pytest.raises(RuntimeError, match="other memory"):
+            ops.tree_attention(q, k, v, lengths, mass=both.view(-1)[8:8 + 54].view(2, 3, 9), out=out)
+        mass = torch.zeros(2, 3, 10)
+        ops.tree_attention(q, k, v, lengths, mass=mass[:, :, 1:])
+        assert torch.allclose(mass.sum(-1), torch.full((2, 3), 4.0), rtol=1e-5) and bool((mass[:, :, 0] == 0).all())
