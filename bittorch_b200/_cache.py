@@ -469,33 +469,45 @@ def _reorder_plan(sigs, parents_sig, len_sig, start):
     if len(shape) != 4 or shape[0] != b * w or 0 in shape or dtype not in _DT:
         _fail(f"cache tensors must be float32, float16 or bfloat16 [{b * w}, Hkv, S, D], got {dtype} {list(shape)}")
     _require(start >= 0, "start must not be negative")
-    strides, spans = [], []
+    strides = []
     for size, stride, kind in sigs:
         if size != shape or kind != dtype:
             _fail("reorder_cache: all cache tensors must have one shape and type")
         if (stride[3] != 1 and shape[3] != 1) or not _plain_memory(torch.empty_strided(size, stride, dtype=kind, device="meta")):
             _fail("reorder_cache: cache tensors must have a contiguous head dimension and share no memory with themselves")
         strides += stride[:3]
-        spans.append(1 + sum((n - 1) * st for n, st in zip(size, stride)))
-    bytes_each = torch.empty(0, dtype=dtype).element_size()
     count = len(sigs)
     return ((count, _DT[dtype], b, w, *shape[1:], (_i64 * (3 * count))(*strides)), _lengths(lengths, b),
-            tuple(n * bytes_each for n in spans), _p * count)
+            [_span(*sig) for sig in sigs], _p * count)
+
+
+@functools.lru_cache(maxsize=64)
+def _views_apart(sigs, offsets) -> bool:
+    """Whether tensors at these distances from the first of them share no memory."""
+    parts = sorted(zip(offsets, sigs), key=lambda x: x[0])
+    for i, (at, sig) in enumerate(parts):
+        end = at + _span(*sig)
+        for other, other_sig in parts[i + 1:]:
+            if other >= end:
+                break
+            if _meet(sig, other_sig, other - at):
+                return False
+    return True
 
 
 def reorder_cache(caches: Sequence[Tensor], parents: Tensor, lengths: Tensor, start: int) -> None:
     start = int(start)
-    head, lens, spans, pointer_array = _reorder_plan(tuple([_sig(c) for c in caches]), _sig(parents), _sig(lengths), start)
+    sigs = tuple([_sig(c) for c in caches])
+    head, lens, spans, pointer_array = _reorder_plan(sigs, _sig(parents), _sig(lengths), start)
     if torch.is_grad_enabled():
         _no_gradient("reorder_cache", *caches)
     index = _same_device("reorder_cache", parents, lengths, *caches)
     pointers = [c.data_ptr() for c in caches]
     if len(pointers) > 1:
-        # tensors of one shape that interleave in memory (views of one buffer) are told apart by their first elements alone
-        ordered = sorted(zip(pointers, spans, caches), key=lambda x: x[0])
-        for (p0, n0, c0), (p1, _, c1) in zip(ordered, ordered[1:]):
-            if p1 == p0 or (p1 - p0 < n0 and c0.is_contiguous() and c1.is_contiguous()):
-                _fail("reorder_cache: a cache tensor is listed twice, or two share memory")
+        # the usual caches lie one behind the other; views of one buffer are looked at element by element
+        ordered = sorted(zip(pointers, spans))
+        if any(p1 - p0 < n0 for (p0, n0), (p1, _) in zip(ordered, ordered[1:])) and not _views_apart(sigs, tuple([p - pointers[0] for p in pointers])):
+            _fail("reorder_cache: a cache tensor is listed twice, or two share memory")
     if not parents.is_contiguous():
         parents = parents.contiguous()
     _call(index, _reorder_cache, pointer_array(*pointers), *head, parents.data_ptr(), lengths.data_ptr(), *lens, start)

@@ -148,3 +148,27 @@ def test_attention_refuses_shared_memory_and_nothing_else(monkeypatch):
         mass = torch.zeros(2, 3, 10)
         ops.tree_attention(q, k, v, lengths, mass=mass[:, :, 1:])
         assert torch.allclose(mass.sum(-1), torch.full((2, 3), 4.0), rtol=1e-5) and bool((mass[:, :, 0] == 0).all())
+
+
+def test_reordering_refuses_views_that_meet(monkeypatch):
+    """Views of one buffer that interleave are taken, strided ones that have elements in common are not."""
+    g = torch.Generator().manual_seed(3)
+    parents, lengths = torch.tensor([[1, 0, 2], [0, 0, 1]]), torch.tensor([5, 7])
+    source = (parents + torch.arange(2)[:, None] * 3).reshape(-1)
+    with on_the_cpu(monkeypatch) as (ops, _):
+        layers = torch.randn(6, 4, 2, 2, 7, 8, generator=g)                 # row, layer, keys or values, head, slot, column
+        views = [layers[:, i, j] for i in range(4) for j in range(2)]
+        before = [x.clone() for x in views]
+        ops.reorder_cache(views, parents, lengths)
+        for x, old in zip(views, before):
+            for row in range(6):
+                n = int(lengths[row // 3])
+                assert torch.equal(x[row, :, :n], old[source[row], :, :n]) and torch.equal(x[row, :, n:], old[row, :, n:])
+        buf = torch.randn(6, 2, 12, 8, generator=g)
+        for first in (0, 1, 5):                                             # they meet in slots first .. 6
+            with pytest.raises(RuntimeError, match="share memory"):
+                ops.reorder_cache([buf[:, :, first:first + 7], torch.randn(6, 2, 7, 8), buf[:, :, :7]], parents, lengths)
+        wide = torch.randn(6, 2, 7, 12, generator=g)
+        with pytest.raises(RuntimeError, match="share memory"):
+            ops.reorder_cache([wide[..., :8], wide[..., 4:]], parents, lengths)
+        ops.reorder_cache([wide[..., :6], wide[..., 6:]], parents, lengths)
