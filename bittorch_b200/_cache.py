@@ -13,6 +13,7 @@ import math
 from typing import Optional, Sequence, Tuple
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 from torch import Tensor
 
 from . import _C
@@ -71,6 +72,8 @@ def _require(ok: bool, text: str) -> None:
 def _no_gradient(what: str, *tensors: Optional[Tensor]) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         _fail(f"{what} has no backward pass: call it under torch.no_grad()")
+    if any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors):      # None outside a dual level
+        _fail(f"{what} has no forward-mode derivative: its output would lose the tangent")
 
 
 def _on_one_device(what: str, *tensors: Optional[Tensor]) -> torch.device:
@@ -262,7 +265,7 @@ def tree_attention(q: Tensor, k: Tensor, v: Tensor, lengths: Tensor, tree: Optio
     if scale is None:
         scale = q.shape[-1] ** -0.5
     plan = _attention_plan(_sig(q), _sig(k), _sig(v), _sig(lengths), _sig(tree), scale, _sig(mass), _sig(out), q.get_device())
-    if torch.is_grad_enabled():
+    if torch.is_grad_enabled() or _forward_ad._current_level >= 0:
         _no_gradient("tree_attention", q, k, v, mass, out)
     index = _same_device("tree_attention", q, k, v, lengths, tree, mass, out)
     head, lens, tree_sb, mass_strides, need, out_strides, spans = plan
@@ -354,7 +357,7 @@ def compact_cache(k: Tensor, v: Tensor, keep: Tensor, counts: Tensor, first: Opt
     head, tail, mass_strides, spans = _compact_plan(_sig(k), _sig(v), _sig(keep), _sig(counts), _sig(first), _sig(mass),
                                                     None if out is None else tuple(_sig(x) for x in out))
     k_out, v_out, mass_out = (k, v, mass) if out is None else (out[0], out[1], out[2] if mass is not None else None)
-    if torch.is_grad_enabled():
+    if torch.is_grad_enabled() or _forward_ad._current_level >= 0:
         _no_gradient("compact_cache", k, v, k_out, v_out, mass, mass_out)
     if not _moves_apart(spans, (k, v) if mass is None else (k, v, mass), out):
         _fail("keys and values (and mass) that share the same memory cannot be compacted in place" if out is None else
@@ -386,7 +389,7 @@ def evict_cache(k: Tensor, v: Tensor, mass: Tensor, lengths: Tensor, budget: int
     (sizes, strides, lens), (head, tail, mass_strides, spans) = _evict_cache_plan(
         _sig(k), _sig(v), _sig(mass), _sig(lengths), budget, sinks, recent, None if out is None else tuple([_sig(x) for x in out]))
     k_out, v_out, mass_out = (k, v, mass) if out is None else out
-    if torch.is_grad_enabled():
+    if torch.is_grad_enabled() or _forward_ad._current_level >= 0:
         _no_gradient("evict_cache", k, v, k_out, v_out, mass, mass_out)
     k_at, v_at, mass_at = k.data_ptr(), v.data_ptr(), mass.data_ptr()
     if not _moves_apart(spans, (k, v, mass), out):
@@ -437,7 +440,7 @@ def _beam_plan(logits_sig, scores_sig, select, finished_sig, end_token):
 def beam_select(logits: Tensor, scores: Tensor, select: Optional[int], finished: Optional[Tensor],
                 end_token: Optional[int]) -> Tuple[Tensor, Tensor, Tensor]:
     head, n, need = _beam_plan(_sig(logits), _sig(scores), select, _sig(finished), end_token)
-    if torch.is_grad_enabled():
+    if torch.is_grad_enabled() or _forward_ad._current_level >= 0:
         _no_gradient("beam_select", logits, scores)
     index = _same_device("beam_select", logits, scores, finished)
     logits = _rows(logits)
@@ -499,7 +502,7 @@ def reorder_cache(caches: Sequence[Tensor], parents: Tensor, lengths: Tensor, st
     start = int(start)
     sigs = tuple([_sig(c) for c in caches])
     head, lens, spans, pointer_array = _reorder_plan(sigs, _sig(parents), _sig(lengths), start)
-    if torch.is_grad_enabled():
+    if torch.is_grad_enabled() or _forward_ad._current_level >= 0:
         _no_gradient("reorder_cache", *caches)
     index = _same_device("reorder_cache", parents, lengths, *caches)
     pointers = [c.data_ptr() for c in caches]

@@ -172,3 +172,27 @@ def test_reordering_refuses_views_that_meet(monkeypatch):
         with pytest.raises(RuntimeError, match="share memory"):
             ops.reorder_cache([wide[..., :8], wide[..., 4:]], parents, lengths)
         ops.reorder_cache([wide[..., :6], wide[..., 6:]], parents, lengths)
+
+
+def test_tangents_are_refused():
+    """Forward-mode differentiation does not show in requires_grad: a dual tensor's tangent must not be lost in silence."""
+    import torch.autograd.forward_ad as fwd
+    from bittorch_b200 import ops
+
+    k, v, mass, n = torch.zeros(2, 3, 10, 8), torch.zeros(2, 3, 10, 8), torch.zeros(2, 3, 10), torch.zeros(2, dtype=torch.int64)
+    q, keep = torch.zeros(2, 3, 1, 8), torch.zeros(2, 3, 4, dtype=torch.int64)
+    x, s, parents = torch.zeros(2, 3, 50), torch.zeros(2, 3), torch.zeros(1, 2, dtype=torch.int64)
+    calls = [(lambda *a: ops.tree_attention(*a, n), (q, k, v)), (lambda a, b: ops.tree_attention(q, a, v, n, mass=b), (k, mass)),
+             (lambda a, b: ops.compact_cache(a, b, keep, n), (k, v)), (lambda *a: ops.evict_cache(*a, n, 4, 1, 1), (k, v, mass)),
+             (ops.beam_select, (x, s)), (lambda a, b: ops.reorder_cache([a, b], parents, n[:1]), (k, v))]
+    for call, args in calls:
+        for i in range(len(args)):
+            for quiet in (False, True):
+                with fwd.dual_level(), torch.set_grad_enabled(not quiet):
+                    dual = [fwd.make_dual(a, torch.ones_like(a)) if j == i else a for j, a in enumerate(args)]
+                    with pytest.raises(RuntimeError, match="forward-mode"):
+                        call(*dual)
+                    with pytest.raises(RuntimeError, match="CUDA"):        # no tangent: as outside a dual level
+                        call(*args)
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(lambda a: ops.tree_attention(a, k, v, n), (q,), (torch.ones_like(q),))
