@@ -57,6 +57,8 @@ _beam_select, _beam_select_workspace = _fn["bt_beam_select"], _fn["bt_beam_selec
 _reorder_cache = _fn["bt_reorder_cache"]
 
 _DT = _C._DT
+# What a call writes in place counts as changed: autograd refuses to go back through a graph that has saved it
+_written = torch.autograd.graph.increment_version
 _SIX, _TWELVE, _FOUR = _i64 * 6, _i64 * 12, _i64 * 4
 
 
@@ -269,9 +271,10 @@ def tree_attention(q: Tensor, k: Tensor, v: Tensor, lengths: Tensor, tree: Optio
         _no_gradient("tree_attention", q, k, v, mass, out)
     index = _same_device("tree_attention", q, k, v, lengths, tree, mass, out)
     head, lens, tree_sb, mass_strides, need, out_strides, spans = plan
-    if out is not None or mass is not None:
-        written = [(t, t.data_ptr(), n) for t, n in ((mass, spans[3]), (out, spans[4])) if t is not None]
-        if not _all_apart(written, [(t, t.data_ptr(), n) for t, n in zip((q, k, v), spans)]):
+    written = [t for t in (mass, out) if t is not None]
+    if written:
+        at = [(t, t.data_ptr(), n) for t, n in ((mass, spans[3]), (out, spans[4])) if t is not None]
+        if not _all_apart(at, [(t, t.data_ptr(), n) for t, n in zip((q, k, v), spans)]):
             _fail("out and mass must be other memory than the queries and the cache, and than each other")
     q = _rows(q)
     if tree is not None and not tree.is_contiguous():
@@ -283,6 +286,8 @@ def tree_attention(q: Tensor, k: Tensor, v: Tensor, lengths: Tensor, tree: Optio
     _call(index, _tree_attention, q.data_ptr(), k.data_ptr(), v.data_ptr(), *head, lengths.data_ptr(), *lens,
           None if tree is None else tree.data_ptr(), tree_sb, scale, None if mass is None else mass.data_ptr(), *mass_strides,
           out.data_ptr(), None if work is None else work.data_ptr(), need)
+    if written:
+        _written(written)
     return out
 
 
@@ -369,6 +374,7 @@ def compact_cache(k: Tensor, v: Tensor, keep: Tensor, counts: Tensor, first: Opt
     _call(index, _compact_cache, k.data_ptr(), v.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), *head, keep.data_ptr(), *tail,
           counts.data_ptr(), None if first is None else first.data_ptr(), None if mass is None else mass.data_ptr(),
           None if mass is None else mass_out.data_ptr(), mass_strides)
+    _written((k_out, v_out) if mass is None else (k_out, v_out, mass_out))
 
 
 @functools.lru_cache(maxsize=1024)
@@ -407,6 +413,7 @@ def evict_cache(k: Tensor, v: Tensor, mass: Tensor, lengths: Tensor, budget: int
     keep_at, counts_at = keep.data_ptr(), counts.data_ptr()
     _call(index, _evict_select, mass_at, *strides, *sizes, lengths.data_ptr(), *lens, budget, sinks, recent, keep_at, counts_at)
     _call(index, _compact_cache, k_at, v_at, k_to, v_to, *head, keep_at, *tail, counts_at, None, mass_at, mass_to, mass_strides)
+    _written((k_out, v_out, mass_out))
     return keep, counts
 
 
@@ -514,3 +521,4 @@ def reorder_cache(caches: Sequence[Tensor], parents: Tensor, lengths: Tensor, st
     if not parents.is_contiguous():
         parents = parents.contiguous()
     _call(index, _reorder_cache, pointer_array(*pointers), *head, parents.data_ptr(), lengths.data_ptr(), *lens, start)
+    _written(caches)

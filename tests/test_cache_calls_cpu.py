@@ -196,3 +196,33 @@ def test_tangents_are_refused():
                         call(*args)
     with pytest.raises(RuntimeError, match="forward-mode"):
         torch.func.jvp(lambda a: ops.tree_attention(a, k, v, n), (q,), (torch.ones_like(q),))
+
+
+def test_what_a_call_writes_counts_as_changed(monkeypatch):
+    """Version counters of the tensors that are written, of those alone; a graph that has saved one refuses to go back."""
+    g = torch.Generator().manual_seed(4)
+    with on_the_cpu(monkeypatch) as (ops, _):
+        k, v, q = torch.randn(2, 3, 10, 8, generator=g), torch.randn(2, 3, 10, 8, generator=g), torch.randn(2, 3, 1, 8, generator=g)
+        mass, n, keep = torch.rand(2, 3, 10, generator=g), torch.tensor([9, 8]), torch.arange(4).expand(2, 3, 4)
+        out, small = torch.empty_like(q), (torch.zeros(2, 3, 5, 8), torch.zeros(2, 3, 5, 8), torch.zeros(2, 3, 5))
+        calls = [(lambda: ops.tree_attention(q, k, v, n), ()), (lambda: ops.tree_attention(q, k, v, n, mass=mass, out=out), (mass, out)),
+                 (lambda: ops.evict_cache(k, v, mass, n, 5, out=small), small), (lambda: ops.evict_cache(k, v, mass, n, 5), (k, v, mass)),
+                 (lambda: ops.compact_cache(k, v, keep, n, out=small[:2]), small[:2]), (lambda: ops.compact_cache(k, v, keep, n), (k, v)),
+                 (lambda: ops.compact_cache(k, v, keep, n, mass=mass), (k, v, mass)),
+                 (lambda: ops.reorder_cache([k, v], torch.tensor([[1, 0]]), n[:1]), (k, v)), (lambda: ops.evict_select(mass, n, 5, 1, 1), ()),
+                 (lambda: ops.beam_select(q[:, :, 0], mass[:, :, 0]), ())]
+        every = (q, k, v, mass, n, out, *small)
+        for call, written in calls:
+            before = [t._version for t in every]
+            call()
+            for t, old in zip(every, before):
+                assert (t._version > old) == any(t is w for w in written)
+        w = torch.ones(8, requires_grad=True)
+        loss = (k * w).sum()                                                # saves k
+        with torch.no_grad():
+            ops.compact_cache(k, v, keep, n)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+        with torch.inference_mode():                                        # tensors without a counter
+            a, b = k.clone(), v.clone()
+            ops.compact_cache(a, b, keep, n)
