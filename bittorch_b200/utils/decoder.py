@@ -491,9 +491,15 @@ class TernaryDecoder(nn.Module):
 
     # ---- serving: trees of drafted tokens, beams, bounded caches (operators over the cache; CUDA only) ----------------
 
+    @torch.no_grad()
     def decode_tokens(self, tokens: Tensor, cache: list, step: CacheStep) -> Tensor:
         """tokens [B, T] at the slots and positions of ``step`` -> logits [B, T, vocab].  Writes the tokens' keys and values
-        to slots ``step.lengths[b] + t``, which the caller keeps inside the cache, and leaves ``step.lengths`` alone."""
+        to slots ``step.lengths[b] + t`` and leaves ``step.lengths`` alone.  Slots and positions that do not exist are
+        refused (which reads them back; while a graph is captured the caller keeps to them)."""
+        self._room(cache, step.lengths, tokens.shape[1], step.positions)
+        return self._decode_tokens(tokens, cache, step)
+
+    def _decode_tokens(self, tokens: Tensor, cache: list, step: CacheStep) -> Tensor:
         x = self.tok(tokens)
         if self._fused_blocks():
             return self._run_fused(x, cache, step, fixed=False)
@@ -501,10 +507,18 @@ class TernaryDecoder(nn.Module):
             x = block.decode_tokens(x, layer_cache, step, self.rope_cos, self.rope_sin)
         return self.head(self.norm(x))
 
-    def _room(self, cache: list, lengths: Tensor, tokens: int) -> None:
-        """Refuses a step that would write past the cache (reads ``lengths`` back, except while a graph is captured)."""
-        slots = cache[0][0].shape[2] if cache else self.cfg.max_seq_len
-        if tokens > slots or (not torch.cuda.is_current_stream_capturing() and int(lengths.max()) + tokens > slots):
+    def _room(self, cache: list, lengths: Tensor, tokens: int, positions: Optional[Tensor] = None) -> None:
+        """Refuses a step that would write outside the cache, or read outside the table of rotations (reads ``lengths`` and
+        ``positions`` back, except while a graph is captured)."""
+        slots = min((layer[0].shape[2] for layer in cache), default=self.cfg.max_seq_len)
+        full = tokens > slots
+        if not full and not (lengths.is_cuda and torch.cuda.is_current_stream_capturing()):
+            ends = [*lengths.aminmax(), *(() if positions is None else positions.aminmax())]
+            least, most, *at = torch.stack([x.long() for x in ends]).tolist()
+            if least < 0 or (at and (at[0] < 0 or at[1] >= self.cfg.max_seq_len)):
+                raise ValueError(f"lengths must not be negative, and positions must be below max_seq_len={self.cfg.max_seq_len}")
+            full = most + tokens > slots
+        if full:
             raise ValueError(f"{tokens} new tokens do not fit behind the filled part of a cache of {slots} slots")
 
     @torch.no_grad()
@@ -515,7 +529,7 @@ class TernaryDecoder(nn.Module):
         self._room(cache, lengths, tokens.shape[1])
         depth = (tree.sum(dim=-1) - 1).clamp(min=0)                              # [T] or [B, T]
         positions = (lengths[:, None] + depth).clamp(max=self.cfg.max_seq_len - 1)
-        return self.decode_tokens(tokens, cache, CacheStep(lengths, positions, tree))
+        return self._decode_tokens(tokens, cache, CacheStep(lengths, positions, tree))
 
     @torch.no_grad()
     def accept_tree(self, tokens: Tensor, parents: Tensor, tree: Tensor, logits: Tensor, cache: list, lengths: Tensor):
@@ -635,7 +649,7 @@ class TernaryDecoder(nn.Module):
             self.forward(prompt[:, :head], [c[:2] for c in full], 0, last_only=True)
         lengths = torch.full((b,), head, dtype=torch.int64, device=dev)
         positions = torch.arange(head, t, device=dev).expand(b, t - head)
-        current = self.decode_tokens(prompt[:, head:], full, CacheStep(lengths, positions))[:, -1].argmax(dim=-1, keepdim=True)
+        current = self._decode_tokens(prompt[:, head:], full, CacheStep(lengths, positions))[:, -1].argmax(dim=-1, keepdim=True)
         lengths = torch.full((b,), t, dtype=torch.int64, device=dev)
         out = [prompt, current]
         cfg = self.cfg
@@ -653,7 +667,7 @@ class TernaryDecoder(nn.Module):
                     _, counts = evict_cache(k, v, m, lengths, budget, sinks, recent)
                 lengths, filled = counts, budget
             positions = torch.full((b, 1), t + i - 1, dtype=torch.long, device=dev)
-            current = self.decode_tokens(current, cache, CacheStep(lengths, positions))[:, -1].argmax(dim=-1, keepdim=True)
+            current = self._decode_tokens(current, cache, CacheStep(lengths, positions))[:, -1].argmax(dim=-1, keepdim=True)
             out.append(current)
             lengths, filled = lengths + 1, filled + 1
         return torch.cat(out[:1 + new_tokens], dim=1)

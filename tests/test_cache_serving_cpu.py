@@ -1,0 +1,47 @@
+"""The decoder's serving paths with the operators' kernels compiled for the CPU: their checks, and decoding within a bounded
+cache against a plain loop."""
+
+import pytest
+import torch
+
+from tests.simt.cache_ops import on_the_cpu
+
+VOCAB = 23
+
+
+def _model(**kw):
+    from bittorch_b200.utils.decoder import DecoderConfig, TernaryDecoder
+
+    torch.manual_seed(0)
+    cfg = dict(vocab_size=VOCAB, dim=32, n_layers=2, n_heads=4, n_kv_heads=2, ffn_dim=48, max_seq_len=40)
+    cfg.update(kw)
+    model = TernaryDecoder(DecoderConfig(backend="python", **cfg)).eval()
+    with torch.no_grad():
+        model.head.weight.mul_(4)                                           # clear choices: a rounding decides no token
+    return model
+
+
+def _prompt(b, t, seed=1):
+    return torch.randint(0, VOCAB, (b, t), generator=torch.Generator().manual_seed(seed))
+
+
+def test_decode_tokens_in_grad_mode_and_outside_the_cache(monkeypatch):
+    """No graph is built, and nothing is written for a step whose slots or positions do not exist."""
+    from bittorch_b200.utils.decoder import CacheStep
+
+    model, prompt, tokens = _model(), _prompt(2, 6), _prompt(2, 3, 2)
+    with on_the_cpu(monkeypatch):
+        cache = model.new_cache(2)
+        with torch.no_grad():
+            want = model(torch.cat([prompt, tokens], 1))[:, 6:]
+            model(prompt, cache, 0)
+        step = lambda at, first: CacheStep(torch.tensor(at), torch.tensor(first)[:, None] + torch.arange(3))
+        before = [x.clone() for layer in cache for x in layer]
+        for at, first in (([6, 38], [6, 6]), ([6, -1], [6, 6]), ([6, 6], [6, 38]), ([6, 6], [-1, 6]), ([40, 40], [6, 6])):
+            with pytest.raises(ValueError, match="do not fit|negative"):
+                model.decode_tokens(tokens, cache, step(at, first))
+        assert all(torch.equal(x, old) for x, old in zip((x for layer in cache for x in layer), before))
+        with torch.enable_grad():
+            got = model.decode_tokens(tokens, cache, step([6, 6], [6, 6]))
+        assert not got.requires_grad and torch.allclose(got, want, rtol=1e-4, atol=1e-4 * float(want.abs().max()))
+        model.decode_tokens(tokens, cache, step([37, 9], [37, 9]))          # up to the last slot
