@@ -591,10 +591,15 @@ class TernaryDecoder(nn.Module):
     @torch.no_grad()
     def generate_beam(self, prompt: Tensor, beams: int, new_tokens: int, end_token: Optional[int] = None) -> Tuple[Tensor, Tensor]:
         """Beam search: prompt [B, T] -> (sequences [B, beams, T + new_tokens], best first, and their log-probabilities
-        float32 [B, beams]).  A beam that has produced ``end_token`` keeps its score and repeats that token."""
+        float32 [B, beams]).  A beam that has produced ``end_token`` keeps its score and repeats that token.  Up to 32 beams
+        (64 for a single new token), and no more than the vocabulary."""
+        from .._cache import BEAM_MAX_SELECT, REORDER_MAX_BEAMS
         from ..ops import beam_select, reorder_cache
 
         b, t = prompt.shape
+        most = min(BEAM_MAX_SELECT if new_tokens == 1 else REORDER_MAX_BEAMS, self.cfg.vocab_size)
+        if not 1 <= beams <= most:
+            raise ValueError(f"beam search takes 1 to {most} beams here, got {beams}")
         if t + new_tokens > self.cfg.max_seq_len:
             raise ValueError(f"positions up to {t + new_tokens} exceed max_seq_len={self.cfg.max_seq_len}")
         if new_tokens < 1:

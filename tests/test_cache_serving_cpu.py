@@ -45,3 +45,19 @@ def test_decode_tokens_in_grad_mode_and_outside_the_cache(monkeypatch):
             got = model.decode_tokens(tokens, cache, step([6, 6], [6, 6]))
         assert not got.requires_grad and torch.allclose(got, want, rtol=1e-4, atol=1e-4 * float(want.abs().max()))
         model.decode_tokens(tokens, cache, step([37, 9], [37, 9]))          # up to the last slot
+
+
+@pytest.mark.parametrize("vocab,beams,new,most", [(70, 33, 2, 32), (70, 64, 5, 32), (70, 65, 1, 64), (5, 6, 1, 5), (5, 6, 3, 5), (70, 0, 3, 32)])
+def test_beam_search_refuses_its_beams_before_it_starts(monkeypatch, vocab, beams, new, most):
+    model = _model(vocab_size=vocab, n_layers=1)
+    monkeypatch.setattr(model, "forward", lambda *a, **k: pytest.fail("the prompt was run"))
+    with pytest.raises(ValueError, match=f"1 to {most} beams"):
+        model.generate_beam(_prompt(1, 3) % vocab, beams, new)
+
+
+def test_beam_search_takes_the_beams_that_it_can(monkeypatch):
+    model = _model(vocab_size=70, n_layers=1)
+    with on_the_cpu(monkeypatch):
+        for beams, new in ((64, 1), (32, 2)):
+            sequences, scores = model.generate_beam(_prompt(1, 3), beams, new)
+            assert sequences.shape == (1, beams, 3 + new) and bool((scores[:, :-1] >= scores[:, 1:]).all())
