@@ -643,8 +643,10 @@ class TernaryDecoder(nn.Module):
         if t + new_tokens > self.cfg.max_seq_len:
             raise ValueError(f"positions up to {t + new_tokens} exceed max_seq_len={self.cfg.max_seq_len}")
         recent = (budget - sinks) // 2 if recent is None else recent
-        if slack < 1:
-            raise ValueError("slack must be at least one slot")
+        if slack < 1 or window < 1:
+            raise ValueError("slack must be at least one slot, and window one token")
+        if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
+            raise ValueError(f"a budget of {budget} slots must be positive and hold {sinks} sinks and {recent} recent slots")
         dev = prompt.device
         full = self.new_cache(b)
         mass = lambda k: torch.zeros(k.shape[:3], dtype=torch.float32, device=dev)

@@ -61,3 +61,12 @@ def test_beam_search_takes_the_beams_that_it_can(monkeypatch):
         for beams, new in ((64, 1), (32, 2)):
             sequences, scores = model.generate_beam(_prompt(1, 3), beams, new)
             assert sequences.shape == (1, beams, 3 + new) and bool((scores[:, :-1] >= scores[:, 1:]).all())
+
+
+@pytest.mark.parametrize("change", [dict(window=0), dict(window=-3), dict(slack=0), dict(budget=0), dict(sinks=-1), dict(recent=-1), dict(recent=11), dict(sinks=13)])
+def test_a_bounded_cache_refuses_its_sizes_before_it_starts(monkeypatch, change):
+    model = _model()
+    for name in ("forward", "new_cache"):
+        monkeypatch.setattr(model, name, lambda *a, **k: pytest.fail("the prompt was run"))
+    with pytest.raises(ValueError, match="window|budget"):
+        model.generate_evicting(_prompt(1, 6), 4, **{**dict(budget=12, sinks=2, window=6, slack=3), **change})
