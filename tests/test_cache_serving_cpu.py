@@ -70,3 +70,88 @@ def test_a_bounded_cache_refuses_its_sizes_before_it_starts(monkeypatch, change)
         monkeypatch.setattr(model, name, lambda *a, **k: pytest.fail("the prompt was run"))
     with pytest.raises(ValueError, match="window|budget"):
         model.generate_evicting(_prompt(1, 6), 4, **{**dict(budget=12, sinks=2, window=6, slack=3), **change})
+
+
+def plain_evicting(model, prompt, new_tokens, budget, sinks, recent, window, slack):
+    """generate_evicting token by token in float64: every layer, sequence and key/value head keeps a list of (rotated key, value,
+    collected weight).  -> (tokens, how often it evicted, smallest relative gap between the lightest slot kept and the
+    heaviest dropped, smallest gap between the two largest logits): the gaps say how far float32 may be off."""
+    import copy
+    import math
+
+    from bittorch_b200.utils.decoder import apply_rope_positions
+    from tests import cache_reference as ref
+
+    model = copy.deepcopy(model).cpu().double()
+    cfg = model.cfg
+    hkv, group = cfg.n_kv_heads, cfg.n_heads // cfg.n_kv_heads
+    out, evictions, gap, margin = [], 0, math.inf, math.inf
+    with torch.no_grad():
+        for b in range(prompt.shape[0]):
+            seq = prompt[b].tolist()
+            state = [[[] for _ in range(hkv)] for _ in model.blocks]
+
+            def feed(token, at):
+                x = model.tok(torch.tensor([[token]]))
+                for block, heads in zip(model.blocks, state):
+                    q, k, v = block.attn._qkv(block.norm1(x))
+                    q, k = (apply_rope_positions(y, model.rope_cos, model.rope_sin, torch.tensor([[at]])) for y in (q, k))
+                    row = []
+                    for h, slots in enumerate(heads):
+                        slots.append([k[0, h, 0], v[0, h, 0], 0.0])
+                        keys, values = torch.stack([s[0] for s in slots]), torch.stack([s[1] for s in slots])
+                        for j in range(group):
+                            p = torch.softmax(keys @ q[0, h * group + j, 0] / math.sqrt(cfg.head_dim), 0)
+                            row.append(p @ values)
+                            if at >= len(prompt[b]) - window:
+                                for s, w in zip(slots, p.tolist()):
+                                    s[2] += w
+                    x = x + block.attn.proj(torch.cat(row)[None, None])
+                    x = x + block.mlp(block.norm2(x))
+                logits = model.head(model.norm(x))[0, 0]
+                top = logits.topk(2).values
+                return int(logits.argmax()), float(top[0] - top[1])
+
+            def evict():
+                nonlocal evictions, gap
+                for heads in state:
+                    for h, slots in enumerate(heads):
+                        mass = torch.tensor([s[2] for s in slots], dtype=torch.float64)
+                        keep = ref.keep_slots(mass, len(slots), budget, sinks, recent)
+                        if len(keep) < len(slots):
+                            evictions += 1
+                            middle = range(sinks, len(slots) - recent)
+                            kept, dropped = [mass[i] for i in middle if i in keep], [mass[i] for i in middle if i not in keep]
+                            if kept:
+                                gap = min(gap, float(min(kept) / max(dropped)) - 1)
+                        heads[h] = [slots[i] for i in keep]
+
+            for at, token in enumerate(seq):
+                nxt, clear = feed(token, at)
+            evict()
+            filled = min(len(seq), budget)
+            for i in range(1, new_tokens + 1):
+                seq.append(nxt)
+                margin = min(margin, clear)
+                if i == new_tokens:
+                    break
+                if filled == budget + slack:
+                    evict()
+                    filled = budget
+                nxt, clear = feed(nxt, len(seq) - 1)
+                filled += 1
+            out.append(seq)
+    return torch.tensor(out), evictions, gap, margin
+
+
+@pytest.mark.parametrize("budget,sinks,recent,window,slack,prompt", [(10, 2, 3, 6, 3, 17), (14, 3, 11, 1, 2, 9)])
+def test_a_bounded_cache_against_the_plain_loop(monkeypatch, budget, sinks, recent, window, slack, prompt):
+    """Lengths, positions, weights and slots through several evictions in place.  Keys, values and weights in float32 are off by
+    about 1e-6 of themselves; the gaps show that no choice of a token or a slot is closer than that."""
+    model = _model()
+    tokens = _prompt(2, prompt, 5)
+    want, evictions, gap, margin = plain_evicting(model, tokens, 14, budget, sinks, recent, window, slack)
+    assert evictions >= 8 and gap > 1e-4 and margin > 1e-4
+    with on_the_cpu(monkeypatch):
+        got = model.generate_evicting(tokens, 14, budget=budget, sinks=sinks, recent=recent, window=window, slack=slack)
+    assert torch.equal(got, want)
