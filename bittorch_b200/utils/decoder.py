@@ -576,6 +576,9 @@ class TernaryDecoder(nn.Module):
         while int(lengths.min()) < total:
             at = lengths.clamp(max=total - 1)                                    # a finished sequence runs along on its last token
             tokens, parents = draft(out[:, :int(lengths.max())], current)
+            # an unused root would keep nothing, again and again; another token there would be taken for a chosen one
+            if tokens.shape[1] == 0 or bool((((tokens[:, 0] != current[:, 0]) | (parents[..., 0] != -1)) & (lengths < total)).any()):
+                raise ValueError("a drafted tree must begin with the current token as its root (parents[..., 0] = -1)")
             t = min(tokens.shape[1], self.cfg.max_seq_len - int(at.max()))
             tokens, parents = tokens[:, :t], parents[..., :t]
             tree = tree_mask(parents)

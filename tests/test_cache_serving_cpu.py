@@ -155,3 +155,39 @@ def test_a_bounded_cache_against_the_plain_loop(monkeypatch, budget, sinks, rece
     with on_the_cpu(monkeypatch):
         got = model.generate_evicting(tokens, 14, budget=budget, sinks=sinks, recent=recent, window=window, slack=slack)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("tokens,parents", [
+    (lambda cur: cur, torch.tensor([-2])), (lambda cur: torch.cat([cur, cur], 1), torch.tensor([[-1, 0], [-2, -1]])),
+    (lambda cur: (cur + 1) % VOCAB, torch.tensor([-1])), (lambda cur: cur[:, :0], torch.zeros(0, dtype=torch.long)),
+])
+def test_a_draft_must_begin_with_the_current_token(monkeypatch, tokens, parents):
+    """A root that is unused keeps nothing (the loop would not end), another token would be taken for the model's choice."""
+    model, calls = _model(n_layers=1), []
+
+    def draft(sequence, current):
+        calls.append(1)
+        assert len(calls) < 30, "no progress"
+        return tokens(current), parents
+
+    with on_the_cpu(monkeypatch):
+        with pytest.raises(ValueError, match="begin with the current token"):
+            model.generate_speculative(_prompt(2, 4), 6, draft)
+
+
+def test_a_finished_sequence_may_have_any_tree(monkeypatch):
+    """What is drafted for a sequence that has its tokens changes nothing."""
+    model = _model(n_layers=1)
+    prompt = _prompt(2, 4)
+    want = model.generate_greedy(prompt, 9)
+
+    def draft(sequence, current):
+        """Right chains of three for the first sequence, which ends early; then an unused root there."""
+        n = (sequence >= 0).sum(1)
+        chain = torch.stack([want[0, (n[0] + i).clamp(max=12)] for i in range(3)])
+        tokens = torch.stack([chain, current[1].expand(3)])
+        tokens[0, 0] = current[0, 0] if n[0] < 13 else 0
+        return tokens, torch.tensor([[-1, 0, 1] if n[0] < 13 else [-2, -2, -2], [-1, -2, -2]])
+
+    with on_the_cpu(monkeypatch):
+        assert torch.equal(model.generate_speculative(prompt, 9, draft), want)
