@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import operator
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -264,8 +265,7 @@ def _attention_plan(q_sig, k_sig, v_sig, len_sig, tree_sig, scale, mass_sig, out
 
 def tree_attention(q: Tensor, k: Tensor, v: Tensor, lengths: Tensor, tree: Optional[Tensor], scale: Optional[float],
                    mass: Optional[Tensor], out: Optional[Tensor]) -> Tensor:
-    if scale is None:
-        scale = q.shape[-1] ** -0.5
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     plan = _attention_plan(_sig(q), _sig(k), _sig(v), _sig(lengths), _sig(tree), scale, _sig(mass), _sig(out), q.get_device())
     if torch.is_grad_enabled() or _forward_ad._current_level >= 0:
         _no_gradient("tree_attention", q, k, v, mass, out)
@@ -426,7 +426,7 @@ def _beam_plan(logits_sig, scores_sig, select, finished_sig, end_token):
     b, w, vocab = logits.shape
     if logits.numel() == 0:
         _fail("logits are empty")
-    n = w if select is None else int(select)
+    n = w if select is None else select
     if scores.dtype is not torch.float32 or scores.shape != (b, w):
         _fail(f"scores must be float32 [{b}, {w}], got {scores.dtype} {list(scores.shape)}")
     if not 1 <= w <= BEAM_MAX_BEAMS:
@@ -446,6 +446,8 @@ def _beam_plan(logits_sig, scores_sig, select, finished_sig, end_token):
 
 def beam_select(logits: Tensor, scores: Tensor, select: Optional[int], finished: Optional[Tensor],
                 end_token: Optional[int]) -> Tuple[Tensor, Tensor, Tensor]:
+    select = None if select is None else int(select)
+    end_token = None if end_token is None else operator.index(end_token)
     head, n, need = _beam_plan(_sig(logits), _sig(scores), select, _sig(finished), end_token)
     if torch.is_grad_enabled() or _forward_ad._current_level >= 0:
         _no_gradient("beam_select", logits, scores)

@@ -226,3 +226,26 @@ def test_what_a_call_writes_counts_as_changed(monkeypatch):
         with torch.inference_mode():                                        # tensors without a counter
             a, b = k.clone(), v.clone()
             ops.compact_cache(a, b, keep, n)
+
+
+def test_numbers_of_any_kind(monkeypatch):
+    """Scales and end tokens as numpy numbers or tensors of one element are taken by their value; nothing is kept of them."""
+    import numpy as np
+    from bittorch_b200 import _cache
+
+    g = torch.Generator().manual_seed(6)
+    with on_the_cpu(monkeypatch) as (ops, _):
+        q, k, v = torch.randn(2, 2, 1, 8, generator=g), torch.randn(2, 2, 9, 8, generator=g), torch.randn(2, 2, 9, 8, generator=g)
+        n, half = torch.tensor([5, 7]), torch.tensor(0.5)
+        want = ops.tree_attention(q, k, v, n, scale=0.5)
+        for scale in (half, torch.tensor([0.5]), np.float32(0.5), np.float64(0.5)):
+            assert torch.equal(ops.tree_attention(q, k, v, n, scale=scale), want)
+        assert _cache._attention_plan.cache_info().currsize == 1
+        half.fill_(float("inf"))
+        with pytest.raises(RuntimeError, match="scale must be finite"):
+            ops.tree_attention(q, k, v, n, scale=half)
+        x, s, done = torch.randn(2, 3, 20, generator=g), torch.randn(2, 3, generator=g), torch.tensor([[True, False, True], [False, True, False]])
+        want = ops.beam_select(x, s, 4, done, 7)
+        for end in (torch.tensor(7), np.int64(7), np.uint8(7)):
+            assert all(torch.equal(a, b) for a, b in zip(ops.beam_select(x, s, np.int32(4), done, end), want))
+        assert _cache._beam_plan.cache_info().currsize == 1
