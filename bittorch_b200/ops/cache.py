@@ -101,7 +101,9 @@ def evict_cache(k_cache: Tensor, v_cache: Tensor, mass: Tensor, lengths: Tensor,
 def beam_select(logits: Tensor, scores: Tensor, select: Optional[int] = None, finished: Optional[Tensor] = None,
                 end_token: Optional[int] = None) -> Tuple[Tensor, Tensor, Tensor]:
     """The ``select`` best continuations (default: as many as beams) of every sequence by ``scores[b, w] +
-    log_softmax(logits[b, w])[v]``, best first; equal scores go to the lowest ``w * V + v``; ranked in float64.
+    log_softmax(logits[b, w])[v]``, best first; equal scores go to the lowest ``w * V + v``.  Sums are ranked in float64; a
+    row's log-sum of exponentials in them is off by 3.3e-6 at most (float32 exponentials; 2e-7 as a rule), so that candidates
+    of different beams that are closer than this may change places.
     logits [B, beams, V], scores float32 [B, beams].  A beam with ``finished[b, w]`` goes on by ``end_token`` alone, its
     score unchanged.  NaN logits, and beams without a finite score or a finite largest logit, count as -infinity.
     -> (scores float32, tokens int64, parents int64), each [B, select]."""

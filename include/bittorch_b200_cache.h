@@ -92,8 +92,9 @@ int bt_compact_cache(const void* k, const void* v, void* k_out, void* v_out, int
 /*
  * One step of beam search: of the candidates (beam w, token v) of sequence b with
  *   score = scores[b,w] + logits[b,w,v] - log(sum_u exp(logits[b,w,u]))
- * the `n` best, best first (equal scores: the lowest w * V + v).  Ranks are taken in
- * float64.  A beam with finished[b,w] != 0 has one candidate, `end_token` with its score
+ * the `n` best, best first (equal scores: the lowest w * V + v).  The sums are ranked in
+ * float64; the log is off by 3.3e-6 at most (float32 exponentials), so candidates of
+ * different beams that are closer than this may change places.  A beam with finished[b,w] != 0 has one candidate, `end_token` with its score
  * unchanged; its others count as -infinity, as do those of a beam whose score is not
  * finite or whose logits have no finite maximum, and NaN logits.
  * logits [B,W,V] of `dtype`, strides (ld_b, ld_w, 1); scores float32 [B,W];
