@@ -75,7 +75,7 @@ def _require(ok: bool, text: str) -> None:
 def _no_gradient(what: str, *tensors: Optional[Tensor]) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         _fail(f"{what} has no backward pass: call it under torch.no_grad()")
-    if any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors):      # None outside a dual level
+    if _forward_ad._current_level >= 0 and any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         _fail(f"{what} has no forward-mode derivative: its output would lose the tangent")
 
 
@@ -141,19 +141,24 @@ def _meet(a_sig, b_sig, distance: int) -> bool:
     return target >= 0 and solve(0, target)
 
 
-def _apart(a, b) -> bool:
-    """Whether two tensors, each given as (tensor, address, span in bytes), share no memory."""
-    return a[1] + a[2] <= b[1] or b[1] + b[2] <= a[1] or not _meet(_sig(a[0]), _sig(b[0]), b[1] - a[1])
+def _behind_one_another(addresses, spans) -> bool:
+    """Whether tensors lie one behind the other: the usual case, in which none shares memory with another."""
+    end = 0
+    for at, span in sorted(zip(addresses, spans)):
+        if at < end:
+            return False
+        end = at + span
+    return True
 
 
-def _all_apart(written, read=()) -> bool:
-    """Whether what a call writes shares no memory with what else it writes or reads."""
-    for i, a in enumerate(written):
-        for b in written[i + 1:]:
-            if not _apart(a, b):
-                return False
-        for b in read:
-            if not _apart(a, b):
+def _apart(sigs, addresses, spans, written: int) -> bool:
+    """Whether the first ``written`` of the tensors share no memory with one another or with the rest, which may share theirs."""
+    if _behind_one_another(addresses, spans):
+        return True
+    for i in range(written):
+        for j in range(i + 1, len(sigs)):
+            distance = addresses[j] - addresses[i]
+            if -spans[j] < distance < spans[i] and _meet(sigs[i], sigs[j], distance):
                 return False
     return True
 
@@ -259,8 +264,10 @@ def _attention_plan(q_sig, k_sig, v_sig, len_sig, tree_sig, scale, mass_sig, out
     sizes = (b, h, hkv, t, s, d)
     with torch.cuda.device(index):                     # the workspace depends on the device's SM count
         need = _tree_attention_workspace(*sizes, code, mass is not None)
-    spans = tuple(0 if sig is None else _span(*sig) for sig in (q_sig, k_sig, v_sig, mass_sig, out_sig))
-    return (code, *sizes, strides), (len64, len_stride), tree_sb, ((0, 0) if mass is None else mass.stride()[:2]), need, out_strides, spans
+    sigs = [sig for sig in (out_sig, mass_sig, q_sig, k_sig, v_sig) if sig is not None]
+    memory = (sigs, [_span(*sig) for sig in sigs])
+    return ((code, *sizes, strides), (len64, len_stride), tree_sb, ((0, 0) if mass is None else mass.stride()[:2]), need, out_strides, memory,
+            _rows(q) is not q)
 
 
 def tree_attention(q: Tensor, k: Tensor, v: Tensor, lengths: Tensor, tree: Optional[Tensor], scale: Optional[float],
@@ -270,13 +277,14 @@ def tree_attention(q: Tensor, k: Tensor, v: Tensor, lengths: Tensor, tree: Optio
     if torch.is_grad_enabled() or _forward_ad._current_level >= 0:
         _no_gradient("tree_attention", q, k, v, mass, out)
     index = _same_device("tree_attention", q, k, v, lengths, tree, mass, out)
-    head, lens, tree_sb, mass_strides, need, out_strides, spans = plan
-    written = [t for t in (mass, out) if t is not None]
-    if written:
-        at = [(t, t.data_ptr(), n) for t, n in ((mass, spans[3]), (out, spans[4])) if t is not None]
-        if not _all_apart(at, [(t, t.data_ptr(), n) for t, n in zip((q, k, v), spans)]):
+    head, lens, tree_sb, mass_strides, need, out_strides, (sigs, spans), copy_q = plan
+    written = None
+    if out is not None or mass is not None:
+        written = [t for t in (out, mass) if t is not None]
+        if not _apart(sigs, [t.data_ptr() for t in (*written, q, k, v)], spans, len(written)):
             _fail("out and mass must be other memory than the queries and the cache, and than each other")
-    q = _rows(q)
+    if copy_q:
+        q = q.contiguous()
     if tree is not None and not tree.is_contiguous():
         tree = tree.contiguous()
     dev = q.device
@@ -286,7 +294,7 @@ def tree_attention(q: Tensor, k: Tensor, v: Tensor, lengths: Tensor, tree: Optio
     _call(index, _tree_attention, q.data_ptr(), k.data_ptr(), v.data_ptr(), *head, lengths.data_ptr(), *lens,
           None if tree is None else tree.data_ptr(), tree_sb, scale, None if mass is None else mass.data_ptr(), *mass_strides,
           out.data_ptr(), None if work is None else work.data_ptr(), need)
-    if written:
+    if written is not None:
         _written(written)
     return out
 
@@ -347,33 +355,31 @@ def _compact_plan(k_sig, v_sig, keep_sig, counts_sig, first_sig, mass_sig, out_s
     keep_strides = _rows(keep).stride()
     strides = _TWELVE(*k.stride()[:3], *v.stride()[:3], *k_out.stride()[:3], *v_out.stride()[:3])
     mass_strides = None if mass is None else _FOUR(*mass.stride()[:2], *mass_out.stride()[:2])
-    spans = [tuple(_span(*sig) for sig in sigs if sig is not None) for sigs in ((k_sig, v_sig, mass_sig), out_sigs or ())]
-    return (_DT[k.dtype], b, hkv, s, s_out, d, strides), (keep_strides[0], keep_strides[1] if keep.shape[1] == hkv else 0, n), mass_strides, spans
-
-
-def _moves_apart(spans, cache, out) -> bool:
-    """Whether a compaction of ``cache`` = (keys, values[, mass]), in place or into ``out``, writes over nothing that it reads."""
-    read = [(t, t.data_ptr(), n) for t, n in zip(cache, spans[0])]
-    return _all_apart(read) if out is None else _all_apart([(t, t.data_ptr(), n) for t, n in zip(out, spans[1])], read)
+    sigs = [*(out_sigs or ()), *(sig for sig in (k_sig, v_sig, mass_sig) if sig is not None)]
+    memory = (sigs, [_span(*sig) for sig in sigs], 2 if mass is None else 3)          # as _apart takes it
+    return ((_DT[k.dtype], b, hkv, s, s_out, d, strides), (keep_strides[0], keep_strides[1] if keep.shape[1] == hkv else 0, n), mass_strides,
+            memory, _rows(keep) is not keep)
 
 
 def compact_cache(k: Tensor, v: Tensor, keep: Tensor, counts: Tensor, first: Optional[Tensor], mass: Optional[Tensor],
                   out: Optional[Sequence[Tensor]]) -> None:
-    head, tail, mass_strides, spans = _compact_plan(_sig(k), _sig(v), _sig(keep), _sig(counts), _sig(first), _sig(mass),
-                                                    None if out is None else tuple(_sig(x) for x in out))
+    head, tail, mass_strides, (sigs, spans, written), copy_keep = _compact_plan(_sig(k), _sig(v), _sig(keep), _sig(counts), _sig(first), _sig(mass),
+                                                                                None if out is None else tuple([_sig(x) for x in out]))
     k_out, v_out, mass_out = (k, v, mass) if out is None else (out[0], out[1], out[2] if mass is not None else None)
     if torch.is_grad_enabled() or _forward_ad._current_level >= 0:
         _no_gradient("compact_cache", k, v, k_out, v_out, mass, mass_out)
-    if not _moves_apart(spans, (k, v) if mass is None else (k, v, mass), out):
+    at = [t.data_ptr() for t in ((k, v) if mass is None else (k, v, mass))]
+    to = at if out is None else [t.data_ptr() for t in out]
+    if not _apart(sigs, at if out is None else to + at, spans, written):
         _fail("keys and values (and mass) that share the same memory cannot be compacted in place" if out is None else
               "out must be other memory than the cache and share none within itself (leave it out to compact in place)")
     index = _same_device("compact_cache", k, v, k_out, v_out, keep, counts, first, mass, mass_out)
-    keep = _rows(keep)
+    if copy_keep:
+        keep = keep.contiguous()
     counts = counts.contiguous()
     first = None if first is None else first.contiguous()
-    _call(index, _compact_cache, k.data_ptr(), v.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), *head, keep.data_ptr(), *tail,
-          counts.data_ptr(), None if first is None else first.data_ptr(), None if mass is None else mass.data_ptr(),
-          None if mass is None else mass_out.data_ptr(), mass_strides)
+    _call(index, _compact_cache, *at[:2], *to[:2], *head, keep.data_ptr(), *tail, counts.data_ptr(), None if first is None else first.data_ptr(),
+          None if mass is None else at[2], None if mass is None else to[2], mass_strides)
     _written((k_out, v_out) if mass is None else (k_out, v_out, mass_out))
 
 
@@ -392,27 +398,26 @@ def _evict_cache_plan(k_sig, v_sig, mass_sig, len_sig, budget, sinks, recent, ou
 def evict_cache(k: Tensor, v: Tensor, mass: Tensor, lengths: Tensor, budget: int, sinks: int, recent: int,
                 out: Optional[Sequence[Tensor]]) -> Tuple[Tensor, Tensor]:
     budget, sinks, recent = int(budget), int(sinks), int(recent)
-    (sizes, strides, lens), (head, tail, mass_strides, spans) = _evict_cache_plan(
+    (sizes, strides, lens), (head, tail, mass_strides, (sigs, spans, written), _) = _evict_cache_plan(
         _sig(k), _sig(v), _sig(mass), _sig(lengths), budget, sinks, recent, None if out is None else tuple([_sig(x) for x in out]))
     k_out, v_out, mass_out = (k, v, mass) if out is None else out
     if torch.is_grad_enabled() or _forward_ad._current_level >= 0:
         _no_gradient("evict_cache", k, v, k_out, v_out, mass, mass_out)
-    k_at, v_at, mass_at = k.data_ptr(), v.data_ptr(), mass.data_ptr()
-    if not _moves_apart(spans, (k, v, mass), out):
+    at = [k.data_ptr(), v.data_ptr(), mass.data_ptr()]
+    to = at if out is None else [k_out.data_ptr(), v_out.data_ptr(), mass_out.data_ptr()]
+    if not _apart(sigs, at if out is None else to + at, spans, written):
         _fail("keys, values and mass that share the same memory cannot be evicted from in place" if out is None else
               "out must be other memory than the cache and share none within itself (leave it out to evict in place)")
     if out is None:
-        k_to, v_to, mass_to = k_at, v_at, mass_at
         index = _same_device("evict_cache", k, v, mass, lengths)
     else:
-        k_to, v_to, mass_to = k_out.data_ptr(), v_out.data_ptr(), mass_out.data_ptr()
         index = _same_device("evict_cache", k, v, mass, lengths, k_out, v_out, mass_out)
     b, hkv, _ = sizes
     keep = torch.empty((b, hkv, budget), dtype=torch.int64, device=k.device)
     counts = torch.empty((b,), dtype=torch.int64, device=k.device)
     keep_at, counts_at = keep.data_ptr(), counts.data_ptr()
-    _call(index, _evict_select, mass_at, *strides, *sizes, lengths.data_ptr(), *lens, budget, sinks, recent, keep_at, counts_at)
-    _call(index, _compact_cache, k_at, v_at, k_to, v_to, *head, keep_at, *tail, counts_at, None, mass_at, mass_to, mass_strides)
+    _call(index, _evict_select, at[2], *strides, *sizes, lengths.data_ptr(), *lens, budget, sinks, recent, keep_at, counts_at)
+    _call(index, _compact_cache, at[0], at[1], to[0], to[1], *head, keep_at, *tail, counts_at, None, at[2], to[2], mass_strides)
     _written((k_out, v_out, mass_out))
     return keep, counts
 
@@ -441,18 +446,19 @@ def _beam_plan(logits_sig, scores_sig, select, finished_sig, end_token):
         if not 0 <= end_token < vocab:
             _fail(f"end_token {end_token} is outside the vocabulary of {vocab}")
     code = _DT[logits.dtype]
-    return (code, b, w, vocab, *_rows(logits).stride()[:2]), n, _beam_select_workspace(b, w, vocab, code, n)
+    return (code, b, w, vocab, *_rows(logits).stride()[:2]), n, _beam_select_workspace(b, w, vocab, code, n), _rows(logits) is not logits
 
 
 def beam_select(logits: Tensor, scores: Tensor, select: Optional[int], finished: Optional[Tensor],
                 end_token: Optional[int]) -> Tuple[Tensor, Tensor, Tensor]:
     select = None if select is None else int(select)
     end_token = None if end_token is None else operator.index(end_token)
-    head, n, need = _beam_plan(_sig(logits), _sig(scores), select, _sig(finished), end_token)
+    head, n, need, copy_logits = _beam_plan(_sig(logits), _sig(scores), select, _sig(finished), end_token)
     if torch.is_grad_enabled() or _forward_ad._current_level >= 0:
         _no_gradient("beam_select", logits, scores)
     index = _same_device("beam_select", logits, scores, finished)
-    logits = _rows(logits)
+    if copy_logits:
+        logits = logits.contiguous()
     if not scores.is_contiguous():
         scores = scores.contiguous()
     if finished is not None and not finished.is_contiguous():
@@ -489,36 +495,21 @@ def _reorder_plan(sigs, parents_sig, len_sig, start):
             _fail("reorder_cache: cache tensors must have a contiguous head dimension and share no memory with themselves")
         strides += stride[:3]
     count = len(sigs)
+    spans = [_span(*sig) for sig in sigs]
     return ((count, _DT[dtype], b, w, *shape[1:], (_i64 * (3 * count))(*strides)), _lengths(lengths, b),
-            [_span(*sig) for sig in sigs], _p * count)
-
-
-@functools.lru_cache(maxsize=64)
-def _views_apart(sigs, offsets) -> bool:
-    """Whether tensors at these distances from the first of them share no memory."""
-    parts = sorted(zip(offsets, sigs), key=lambda x: x[0])
-    for i, (at, sig) in enumerate(parts):
-        end = at + _span(*sig)
-        for other, other_sig in parts[i + 1:]:
-            if other >= end:
-                break
-            if _meet(sig, other_sig, other - at):
-                return False
-    return True
+            spans, _p * count, functools.lru_cache(maxsize=16)(lambda offsets: _apart(sigs, offsets, spans, count)))
 
 
 def reorder_cache(caches: Sequence[Tensor], parents: Tensor, lengths: Tensor, start: int) -> None:
     start = int(start)
-    sigs = tuple([_sig(c) for c in caches])
-    head, lens, spans, pointer_array = _reorder_plan(sigs, _sig(parents), _sig(lengths), start)
+    head, lens, spans, pointer_array, views_apart = _reorder_plan(tuple([_sig(c) for c in caches]), _sig(parents), _sig(lengths), start)
     if torch.is_grad_enabled() or _forward_ad._current_level >= 0:
         _no_gradient("reorder_cache", *caches)
     index = _same_device("reorder_cache", parents, lengths, *caches)
     pointers = [c.data_ptr() for c in caches]
     if len(pointers) > 1:
-        # the usual caches lie one behind the other; views of one buffer are looked at element by element
-        ordered = sorted(zip(pointers, spans))
-        if any(p1 - p0 < n0 for (p0, n0), (p1, _) in zip(ordered, ordered[1:])) and not _views_apart(sigs, tuple([p - pointers[0] for p in pointers])):
+        # views of one buffer are looked at element by element, once for their distances
+        if not _behind_one_another(pointers, spans) and not views_apart(tuple([p - pointers[0] for p in pointers])):
             _fail("reorder_cache: a cache tensor is listed twice, or two share memory")
     if not parents.is_contiguous():
         parents = parents.contiguous()
