@@ -73,8 +73,10 @@ def _require(ok: bool, text: str) -> None:
 
 
 def _no_gradient(what: str, *tensors: Optional[Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        _fail(f"{what} has no backward pass: call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                _fail(f"{what} has no backward pass: call it under torch.no_grad()")
     if _forward_ad._current_level >= 0 and any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         _fail(f"{what} has no forward-mode derivative: its output would lose the tangent")
 
