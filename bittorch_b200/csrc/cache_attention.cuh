@@ -11,6 +11,10 @@
 // and the join.  16 rows x 32 slots per step: each thread owns the scores of one slot for four rows, then four
 // rows x four columns of the output.  Bound by shared-memory reads of the two products; the kernels of the files beside it
 // take the calls whose rows can be read in vectors, this one what is left.
+//
+// With mass every score is kept in float32 and read once more by attn_merge, which needs the row's sum over all runs first:
+// 4 sequences of 32776 slots, 64 heads over 8, one token 118 us, 22 us of them for that; 32 tokens over 8190 slots (256 rows a head,
+// 16 at a time, the scores 268 MB) 488 us.
 #pragma once
 
 #include "cache_common.cuh"

@@ -9,7 +9,9 @@
 // take other slots.  Measured against the kernel that stages the cache in shared memory (8 sequences, 8 key/value heads of
 // size 128, 4091 slots): one row 50 us instead of 185 us (5.3 TB/s: HBM), 20 rows 247 us instead of 324 us (10.9 TFLOP/s: the eight
 // warps that fit an SM at 252 registers a thread do not cover the way of the loads; more slots a step and loads a step ahead
-// were slower, 286 us and 277 us).
+// were slower, 286 us and 277 us).  Many rows read the cache again for every 16 of them: 8 sequences of 4000 slots, 64 heads over 8,
+// size 128: 64 rows 736 us, 488 rows 4.4 ms, 14.9 TFLOP/s of 74; two library products with the scores written out between them take
+// 733 us and 3.4 ms.
 #pragma once
 
 #include "cache_attention.cuh"

@@ -15,7 +15,9 @@
 //
 // 32 sequences of 601 to 2303 slots, 20 heads, head size 128, bf16: 90 us with the join, 5.3 TB/s (a plain copy: 6.53).  Head
 // sizes between those it is built for are padded with zeros in the ring: 8 x 4090 slots, 32 heads over 8, head size 80: 38 us,
-// on the CUDA cores 143 us.
+// on the CUDA cores 143 us.  Many rows of a head size other than 64 and 128 are this kernel's too, and the cache is read again, out of
+// L2, for every 16 of them: 8 trees of 61 nodes, 64 heads over 8, up to 8190 slots, bf16: size 80 789 us, 96 764 us, 256 2649 us,
+// 75 to 97 TFLOP/s (size 128 on the tensor-memory kernel 135 us).
 #pragma once
 
 #include "cache_attention.cuh"

@@ -21,10 +21,12 @@
 // they are multiplied, and so are infinities and NaN among the new tokens' values, which are added at the end to
 // the rows that see them.
 //
-// 8 trees of 61 nodes over 4099 to 8190 slots, 64 heads over 8, head size 128, fp16: 127 us, 780 TFLOP/s.  A block of two tiles
-// takes about 3350 cycles; its four products need 2048, the 32768 exponentials of the two streams as many (16 a cycle), and
-// the maxima, conversions and TMEM transfers share the issue slots with them: bound by the streams' issue.  Short calls:
-// by 16 to 19 thousand cycles at the end of a pair (output through shared memory, the pieces' join).
+// 8 trees of 61 nodes over 4099 to 8190 slots, 64 heads over 8, head size 128, fp16: 126 us, 787 TFLOP/s.  A block of two tiles
+// takes about 3350 cycles; its four products need 2048, the 32768 exponentials of the two streams as many (16 a cycle).
+// Bound by latency: the tensor pipe is busy 50 % of the time, the exponentials' pipe 50 %, 37 % of the issue slots are used, and
+// in 63 % of the cycles no warp of a scheduler can issue (11 warps an SM, one thread a row; the streams pass one buffer of
+// scores between them, so that neither's products run while both wait).  Short calls: by 16 to 19 thousand cycles at the
+// end of a pair (output through shared memory, the pieces' join).
 #pragma once
 
 #include "cache_attention_stream.cuh"
